@@ -913,7 +913,12 @@ extern "C" bool qw_buf_upload(qw_buf b, size_t off, const void *src, size_t len)
     if (!b || b->kind == BUF_ARENA || b->kind == BUF_POOL || off + len > b->len) { set_error("qw_buf_upload: bad range"); return false; }
     use_device(b->device);
     if (b->kind == BUF_SHARED) memcpy((char *)b->host + off, src, len);
-    if (cudaMemcpy((char *)b->dev + off, src, len, cudaMemcpyHostToDevice) != cudaSuccess) { set_error("qw_buf_upload: copy failed"); return false; }
+    // (from pageable memory cudaMemcpy returns once the bytes are staged: the wait is for the last of them to have landed,
+    // since command buffers run on streams that do not order with the default one)
+    if (cudaMemcpy((char *)b->dev + off, src, len, cudaMemcpyHostToDevice) != cudaSuccess || cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess) {
+        set_error("qw_buf_upload: copy failed");
+        return false;
+    }
     return true;
 }
 extern "C" bool qw_buf_download(qw_buf b, size_t off, void *dst, size_t len) {
@@ -1010,6 +1015,8 @@ static bool kv_rw(qw_buf cache, int32_t layer, int32_t head, int32_t pos0, int32
             t += cnt;
             hp += (size_t)cnt * row;
         }
+        // (as in qw_buf_upload: the last rows have landed before a command buffer can read them)
+        if (store && cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess) { set_error("qw_kv_store: copy failed"); return false; }
         return true;
     }
     const size_t off = (((size_t)layer * kv_heads + head) * max_ctx + pos0) * row;
