@@ -13,8 +13,11 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("QWASAR_CUDA_LIB") or os.path.join(HERE, "libqwasar_cuda.so")   # (the override: for comparing two builds)
 HEADER = os.path.join(os.path.dirname(HERE), "include", "qwasar_cuda.h")
+KV8_HEADER = os.path.join(os.path.dirname(HERE), "include", "qwasar_kv8.h")
 
 F32, BF16 = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BANDS = 0, 1, 2, 3
 
 
 class QwRef(C.Structure):
@@ -125,6 +128,20 @@ SIGNATURES = {
     "qw_attn_decode_noalloc_status": (_i32, []),
 }
 
+# name -> (restype, argtypes); every symbol include/qwasar_kv8.h declares
+KV8_SIGNATURES = {
+    "qw_op_rope": (_b, [_vp] + [QwRef] * 4 + [_i32] * 4 + [C.c_int, C.c_int64, C.c_int64, _f32, C.c_int]),
+    "qw_rope_scaled_tables": (_b, [_vp, _vp, _i32, _f32, C.c_int, _f32, _i32, _f32, _f32]),
+    "qw_kv8_layer_bytes": (_sz, [_i32, _i32, _i32]),
+    "qw_kv8_arena_alloc": (_vp, [_i32, _i32, _i32, _i32, C.c_uint32]),
+    "qw_kv8_arena_alloc_in": (_vp, [_vp, _i32, _i32, _i32, _i32]),
+    "qw_op_kv8_write": (_b, [_vp] + [QwRef] * 4 + [_i32] * 5 + [C.c_int64, C.c_int]),
+    "qw_op_kv8_write_batch": (_b, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, C.c_int64, C.c_int]),
+    "qw_op_kv8_read": (_b, [_vp, QwRef, QwRef] + [_i32] * 5 + [C.c_int]),
+    "qw_op_attn_kv8": (_b, [_vp] + [QwRef] * 5 + [_i32] * 6 + [_f32, _i32, C.c_int]),
+    "qw_op_attn_kv8_batch": (_b, [_vp, _i32] + [_vp] * 6 + [_i32] * 5 + [_f32, _i32, C.c_int]),
+}
+
 
 def build_library(verbose: bool = False) -> str:
     """Compiles csrc/ for sm_100a with nvcc (works without a GPU)."""
@@ -138,7 +155,7 @@ def load_library() -> C.CDLL:
         raise FileNotFoundError(
             f"{LIB_PATH} is not built; run `make -C qwasar_b200/csrc` (there is no fallback path)")
     lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in (*SIGNATURES.items(), *KV8_SIGNATURES.items()):
         fn = getattr(lib, name)          # AttributeError if the library lacks a declared symbol
         fn.restype, fn.argtypes = res, args
     return lib
@@ -253,6 +270,30 @@ class Backend:
             raise MemoryError(self.last_error())
         return b
 
+    # -- the 8-bit cache
+    def kv8_layer_bytes(self, kv_heads, max_ctx, head_dim=256):
+        return int(self.lib.qw_kv8_layer_bytes(kv_heads, max_ctx, head_dim))
+
+    def kv8_arena_alloc(self, n_layers, kv_heads, max_ctx, head_dim=256, shuffle_seed=0):
+        b = self.lib.qw_kv8_arena_alloc(n_layers, kv_heads, max_ctx, head_dim, shuffle_seed)
+        if not b:
+            raise MemoryError(self.last_error())
+        return b
+
+    def kv8_arena_alloc_in(self, pool, n_layers, kv_heads, max_ctx, head_dim=256):
+        b = self.lib.qw_kv8_arena_alloc_in(pool, n_layers, kv_heads, max_ctx, head_dim)
+        if not b:
+            raise MemoryError(self.last_error())
+        return b
+
+    def rope_scaled_tables(self, rotary_dim, theta, kind=ROPE_PLAIN, factor=1.0, original_ctx=0, beta_fast=32.0, beta_slow=1.0):
+        """(inv_freq float32 [rotary_dim / 2], amp)."""
+        import numpy as np
+        inv, amp = np.empty(max(rotary_dim, 0) // 2, np.float32), C.c_float(1.0)
+        if not self.lib.qw_rope_scaled_tables(inv.ctypes.data, C.addressof(amp), rotary_dim, theta, kind, factor, original_ctx, beta_fast, beta_slow):
+            raise ValueError(self.last_error())
+        return inv, amp.value
+
     # -- the exchange of partials between GPUs
     def xchg_create(self, n_ranks, rank, max_rows_heads):
         x = self.lib.qw_xchg_create(n_ranks, rank, max_rows_heads)
@@ -351,6 +392,22 @@ class Backend:
             c, x, phase, n, C.addressof(arrs[0]), C.addressof(arrs[1]) if gates else None, C.addressof(arrs[2]),
             C.addressof(arrs[3]), C.addressof(arrs[4]), C.addressof(ints[0]), C.addressof(ints[1]), C.addressof(ints[2]),
             rows, q_heads, kv_heads, head_dim, max_ctx, scale, q_dtype, out_dtype, gate_dtype, gate_stride)
+
+    def op_kv8_write_batch(self, c, kcs, vcs, ks, vs, base_pos, rows, kv_heads, head_dim, max_ctx, row_stride, io):
+        n = len(kcs)
+        bp = (C.c_int32 * n)(*base_pos)
+        arrs = [_ref_array(x) for x in (kcs, vcs, ks, vs)]
+        return self.lib.qw_op_kv8_write_batch(c, n, *[C.addressof(a) for a in arrs], C.addressof(bp), rows, kv_heads, head_dim,
+                                              max_ctx, row_stride, io)
+
+    def op_attn_kv8_batch(self, c, outs, gates, qs, kcs, vcs, base_pos, rows, q_heads, kv_heads, head_dim, max_ctx, scale,
+                          gate_stride, io):
+        n = len(outs)
+        bp = (C.c_int32 * n)(*base_pos)
+        arrs = [_ref_array(x) for x in (outs, gates if gates else [NULL_REF] * n, qs, kcs, vcs)]
+        return self.lib.qw_op_attn_kv8_batch(c, n, C.addressof(arrs[0]), C.addressof(arrs[1]) if gates else None,
+                                             C.addressof(arrs[2]), C.addressof(arrs[3]), C.addressof(arrs[4]), C.addressof(bp),
+                                             rows, q_heads, kv_heads, head_dim, max_ctx, scale, gate_stride, io)
 
     def op_attn_batch(self, c, outs, qs, kcs, vcs, base_pos, rows, q_heads, kv_heads, head_dim, max_ctx, scale, io):
         n = len(outs)

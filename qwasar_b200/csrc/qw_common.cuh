@@ -9,6 +9,10 @@
 #define QW_PAGE_TOKENS 64        // tokens per arena page: 64 x 512 B = 32 KB, 128 B-aligned rows
 #define QW_MAX_SEQ 64            // sequences (or row chunks) one launch carries
 #define QW_XCHG_REC 264          // floats per exchanged partial: acc[256], max, sum, padding to 16 bytes
+#define QW_KV8_PAGE_TOKENS 128   // tokens per page of an 8-bit arena: 128 x 256 B = the same 32 KB
+#define QW_KV8_BLOCK 64          // tokens of one head that share an exponent in an 8-bit cache
+#define QW_KV8_E_MIN (-60)       // exponents of an 8-bit cache are kept in this range (a block of zeros has the lowest)
+#define QW_KV8_E_MAX 119
 #define QW_MAX_MAPS 8            // distinct cache tensor maps one launch carries (arenas of one pool share theirs)
 
 // Status codes a kernel leaves in the backend's status word (first one wins).
@@ -20,6 +24,7 @@ enum : int {
     QW_ST_BAD_PAGE = 4,          // a page-table entry was unmapped where a key was needed
     QW_ST_BAD_SMEM = 5,          // the dynamic shared-memory window was not 1024-byte aligned
     QW_ST_PEER_TIMEOUT = 6,      // a partial from another GPU did not arrive within the exchange's time limit
+    QW_ST_KV8_NONFINITE = 7,     // a key or value given to the 8-bit cache was NaN or infinite
 };
 
 namespace qw {

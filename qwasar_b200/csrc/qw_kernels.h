@@ -215,6 +215,71 @@ void launch_qsa_scores(cudaStream_t s, float *scores, const float *qn, const flo
 void launch_qsa_select(cudaStream_t s, uint8_t *mask, uint32_t *list, const float *scores, int rows, int ratio, int base_pos,
                        int block_topk, int max_ctx, int max_blocks);
 
+// ---- rotary positions (qw_rope.cu) -------------------------------------------------------------
+struct RopeParams {
+    void *y;                 // [rows] rows of heads * head_dim elements, y_stride apart
+    const void *x;
+    const int32_t *pos;      // [rows]
+    const float *inv_freq;   // [rotary_dim / 2]
+    int64_t y_stride, x_stride;
+    int32_t rows, heads, head_dim, rotary_dim;
+    int32_t interleaved, io;
+    float amp;
+};
+void launch_rope(cudaStream_t s, const RopeParams &p);
+
+// ---- the 8-bit K/V cache (qw_kv8.cu) ------------------------------------------------------------
+// Where one layer's K (or V) codes and exponents live.  Code row `row(h, t)` is a 256-byte row:
+//   linear: row = h * max_ctx + t;   paged: row = table[h * pt_stride + t / 128] * 128 + t % 128
+// The exponent byte of head h's block b (tokens [64 b, 64 b + 64)) is exps[h * exp_stride + b].
+struct Kv8Layer {
+    uint8_t *base;
+    const int32_t *table;    // nullptr: linear
+    uint8_t *exps;
+    int32_t pt_stride, max_ctx, exp_stride;
+};
+struct Kv8WriteSeq {
+    Kv8Layer kc, vc;
+    const void *k, *v;       // rows of kv_heads * 256 elements, row_stride apart
+    int32_t base_pos;
+};
+struct Kv8WriteParams {
+    Kv8WriteSeq seq[QW_MAX_SEQ];
+    int64_t row_stride;
+    int32_t n_seq, rows, kv_heads, max_blocks;   // max_blocks: blocks of 64 tokens any sequence touches
+    int32_t io;
+    int *status;
+};
+void launch_kv8_write(cudaStream_t s, const Kv8WriteParams &p);
+// dst [kv_heads, n, 256] in `io` = values of positions [pos0, pos0 + n); pages never mapped read as zeros.
+void launch_kv8_read(cudaStream_t s, void *dst, int io, const Kv8Layer &c, int kv_heads, int pos0, int n);
+
+struct Kv8AttnSeq {
+    const void *q;           // [rows, q_heads, 256]
+    void *out;
+    const void *gate;        // nullptr, or element (r, h, d) at gate[(r*q_heads + h)*gate_stride + d]
+    Kv8Layer kc, vc;
+    int32_t rows, base_pos;  // row r reads keys [0, base_pos + r]
+    int32_t n_tiles;         // 32-key tiles per kv head
+    int32_t cum_tiles;       // tiles of all earlier sequences times kv_heads
+    uint8_t kmap, vmap;
+};
+struct Kv8AttnParams {
+    CUtensorMap maps[QW_MAX_MAPS];     // code rows, boxes of 128 bytes x 32 rows, SWIZZLE_128B
+    Kv8AttnSeq seq[QW_MAX_SEQ];
+    int32_t n_seq, q_heads, kv_heads, gqa;
+    int32_t total_tiles, n_cta, slot_rows;
+    int32_t io, gate_stride;
+    float scale;
+    float *pacc, *pstat;     // partials: [slot, slot_rows, 256] and [slot, slot_rows, 2]; slot = cta + group
+    int *status;
+};
+// Query rows (rows * gqa) one sequence of a launch may have.
+inline int kv8_max_query_rows(int io) { return io == DT_F32 ? 32 : 64; }
+void kv8_attn_plan(Kv8AttnParams &p);
+size_t kv8_attn_scratch_bytes(const Kv8AttnParams &p);
+void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scratch);
+
 int sm_count();
 
 

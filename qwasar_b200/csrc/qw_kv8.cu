@@ -1,0 +1,776 @@
+// The 8-bit K/V cache: append, dequantising read, and attention over it (sm_100a).
+//
+// Format.  A key or value element is an e4m3 code times 2^e, with one e per 64 tokens of one head.  e is the
+// smallest whole number for which the block's largest magnitude is at most 448 * 2^e, within [-60, 119]; its byte is
+// e + 127.  Powers of two keep every step but the rounding to e4m3 exact: scaling by 2^-e, moving a block to a larger
+// e when a bigger row arrives (a shift, exact until a code falls below the normal range), widening a code to fp16 or
+// bf16 -- so attention can fold the exponents into the softmax instead of touching the elements.
+#include "qw_kernels.h"
+#include <algorithm>
+#include <cuda_fp16.h>
+
+namespace qw {
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int BLK = QW_KV8_BLOCK;
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // e in [-126, 127]
+__device__ __forceinline__ int clamp_exp(int byte) { return min(max(byte - 127, QW_KV8_E_MIN), QW_KV8_E_MAX); }
+__device__ __forceinline__ int needed_exp(float amax) {
+    // 448 = 1.75 * 2^8
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, QW_KV8_E_MIN), QW_KV8_E_MAX);
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t e4m3x4(const float *v) { return e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16); }
+// two codes -> two fp16 values (exact)
+__device__ __forceinline__ uint32_t f16x2_lo(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2_hi(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+__device__ __forceinline__ float2 h2f2(uint32_t h) {
+    const __half2 v = *reinterpret_cast<const __half2 *>(&h);
+    return __half22float2(v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Row of codes that holds (head, token), or -1 where no page is mapped.
+__device__ __forceinline__ int64_t code_row(const Kv8Layer &L, int h, int t) {
+    if (!L.table) return (int64_t)h * L.max_ctx + t;
+    const int pg = __ldg(L.table + (size_t)h * L.pt_stride + t / QW_KV8_PAGE_TOKENS);
+    return pg < 0 ? -1 : (int64_t)pg * QW_KV8_PAGE_TOKENS + (t & (QW_KV8_PAGE_TOKENS - 1));
+}
+
+// =======================================================================================
+// append
+// =======================================================================================
+// One CTA per (64-token block, head, K or V, sequence): the block's new rows are read once into registers, their
+// largest magnitude gives the exponent, and the codes leave as whole 256-byte rows.  A block that holds rows already
+// keeps its exponent unless the new rows need a larger one; then its old codes are moved there first.
+constexpr int WR_THREADS = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(WR_THREADS) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
+    __shared__ float red[WR_THREADS / 32];
+    pdl_wait();
+    pdl_launch_next();
+    const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const Kv8WriteSeq &sq = p.seq[blockIdx.z];
+    const int blk = sq.base_pos / BLK + (int)blockIdx.x, t0 = blk * BLK;
+    const int first = max(t0, sq.base_pos), last = min(t0 + BLK, sq.base_pos + p.rows);   // new rows of this block
+    if (first >= last) return;
+    const Kv8Layer &L = which ? sq.vc : sq.kc;
+    const T *src = reinterpret_cast<const T *>(which ? sq.v : sq.k) + (size_t)h * 256;
+    const int64_t row0 = code_row(L, h, t0);                 // a block never crosses a page
+    if (row0 < 0) { if (threadIdx.x == 0) report(p.status, QW_ST_BAD_PAGE); return; }
+    uint8_t *dst = L.base + row0 * 256;
+    uint8_t *ep = L.exps + (size_t)h * L.exp_stride + blk;
+    const int col = (threadIdx.x & 31) * 8, r0 = threadIdx.x >> 5;
+
+    float v[8][8];
+    float amax = 0.0f;
+    bool odd = false;                                        // a NaN or an infinity was seen
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int t = first + r0 + 8 * i;
+        if (t < last) {
+            const T *g = src + (size_t)(t - sq.base_pos) * p.row_stride + col;
+            if constexpr (sizeof(T) == 2) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(g);
+                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) { v[i][2 * e] = __uint_as_float(w[e] << 16); v[i][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+            } else {
+                const float4 a = *reinterpret_cast<const float4 *>(g), b = *reinterpret_cast<const float4 *>(g + 4);
+                v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+                v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float a = fabsf(v[i][e]);
+                if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
+                else { odd = true; if (a != a) v[i][e] = 0.0f; }       // NaN: stored as zero; infinite: the largest code
+            }
+        }
+    }
+    if (odd) report(p.status, QW_ST_KV8_NONFINITE);
+    amax = warp_max(amax);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    // (every thread reads the stored exponent before the barrier behind which one of them may replace it)
+    const int was = first > t0 ? clamp_exp(*ep) : QW_KV8_E_MIN;
+    __syncthreads();
+    amax = red[0];
+#pragma unroll
+    for (int i = 1; i < WR_THREADS / 32; i++) amax = fmaxf(amax, red[i]);
+    const int e = max(was, needed_exp(amax));
+    if (first > t0 && e > was) {
+        // rows [t0, first): 16 codes to a thread
+        const float f = pow2f(max(was - e, -126));
+        for (int i = threadIdx.x; i < (first - t0) * 16; i += WR_THREADS) {
+            uint4 *at = reinterpret_cast<uint4 *>(dst + (size_t)i * 16);
+            uint4 q = *at;
+            uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float2 a = h2f2(f16x2_lo(w[k])), b = h2f2(f16x2_hi(w[k]));
+                w[k] = e4m3x2(a.x * f, a.y * f) | (e4m3x2(b.x * f, b.y * f) << 16);
+            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    const float inv = pow2f(-e);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int t = first + r0 + 8 * i;
+        if (t < last) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[i][k] *= inv;
+            *reinterpret_cast<uint2 *>(dst + (size_t)(t - t0) * 256 + col) = make_uint2(e4m3x4(v[i]), e4m3x4(v[i] + 4));
+        }
+    }
+    if (threadIdx.x == 0) *ep = (uint8_t)(e + 127);
+}
+
+// =======================================================================================
+// dequantising read
+// =======================================================================================
+// A warp takes whole rows (32 lanes x 8 codes), eight of them in flight; 1 byte in, 2 or 4 out per element, so the
+// stores are what bounds it.
+constexpr int RD_THREADS = 256, RD_ROWS = 8;     // rows a warp has in flight
+
+template <typename T>
+__global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(T *__restrict__ dst, const Kv8Layer L, int pos0, int n) {
+    pdl_wait();
+    pdl_launch_next();
+    const int h = blockIdx.y, lane = threadIdx.x & 31;
+    const int r0 = ((int)blockIdx.x * (RD_THREADS / 32) + (int)(threadIdx.x >> 5)) * RD_ROWS;
+    uint2 q[RD_ROWS];
+    float s[RD_ROWS];
+#pragma unroll
+    for (int i = 0; i < RD_ROWS; i++) {
+        q[i] = make_uint2(0, 0); s[i] = 0.0f;
+        if (r0 + i < n) {
+            const int t = pos0 + r0 + i;
+            const int64_t row = code_row(L, h, t);
+            if (row >= 0) {
+                q[i] = *reinterpret_cast<const uint2 *>(L.base + row * 256 + lane * 8);
+                s[i] = pow2f(clamp_exp(L.exps[(size_t)h * L.exp_stride + t / BLK]));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RD_ROWS; i++) {
+        if (r0 + i >= n) break;
+        float2 v[4] = {h2f2(f16x2_lo(q[i].x)), h2f2(f16x2_hi(q[i].x)), h2f2(f16x2_lo(q[i].y)), h2f2(f16x2_hi(q[i].y))};
+#pragma unroll
+        for (int k = 0; k < 4; k++) { v[k].x *= s[i]; v[k].y *= s[i]; }
+        T *o = dst + ((size_t)h * n + r0 + i) * 256 + lane * 8;
+        if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint4 *>(o) = make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y), pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
+        } else {
+            *reinterpret_cast<float4 *>(o) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            *reinterpret_cast<float4 *>(o + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        }
+    }
+}
+
+// =======================================================================================
+// attention, few query rows: split over the keys
+// =======================================================================================
+// All (sequence, kv head) groups of a launch lie end to end as one line of 32-key tiles, cut into equal shares, one
+// per CTA (one CTA per SM); a share that crosses a group's end is taken as two segments.  Warp (mt, kg) of a CTA owns
+// 16 rows of the tensor op and every KG-th tile of the segment; the MT warps of one kg read the same tiles.
+//
+// Rows.  Query row i = r * gqa + g of the group (all query heads of the kv head).  fp16 tensor ops, because an e4m3
+// code is an fp16 number exactly.  bf16 rows are exact in fp16 after scaling by a power of two; 16 of them fill a row
+// tile.  f32 rows are cut into a high and a low fp16 part (22 bits), eight rows to a tile: row i's high part in tensor
+// row i, its low part in tensor row i + 8 -- the two sums land in one thread, which adds them.  The softmax weights
+// are cut the same way.  (Weights run up to 2^14, not 1, so that the small ones of a long context stay above fp16's
+// smallest number: 2^-38 of the largest.)
+//
+// Exponents.  A tile of 32 keys has one exponent for K and one for V.  With t = scale * log2(e) * 2^ek * (q . ck) + ev
+// and m the running maximum of t, w = 2^(t - m) weighs the V CODES: o = sum w cv, and the denominator is
+// l = sum w 2^-ev.  Both see each element once, as it lies in the cache.
+//
+// Loads.  Each kg group has a ring of 8 KB slots (K or V of one 32-key tile: two boxes of 128 bytes x 32 rows,
+// SWIZZLE_128B), filled by its first warp as the slots fall free; there is no producer warp, since eight consumer
+// warps with 255 registers each take the whole register file.
+constexpr int AT_THREADS = 256, AT_WARPS = 8;
+constexpr int TILE = 32;
+constexpr int ENTRY = TILE * 256;                    // K or V codes of a tile
+constexpr int BOX = TILE * 128;
+constexpr int RING = 24;                             // slots of a CTA
+constexpr int OFF_Q = RING * ENTRY;
+constexpr float W_SHIFT = 14.0f;
+
+template <int MT>
+struct AtCfg {
+    static constexpr int KG = AT_WARPS / MT;
+    static constexpr int NS = RING / KG;                         // slots of one kg group
+    static constexpr int LAG = MT > 1 ? 2 : 0;                   // entries the loader lets the other warps fall behind
+    static constexpr int OFF_M = OFF_Q + MT * 8192;              // [KG][MT * 16]
+    static constexpr int OFF_L = OFF_M + AT_WARPS * 64;
+    static constexpr int OFF_QE = OFF_L + AT_WARPS * 64;         // [MT * 16] row exponents
+    static constexpr int OFF_META = OFF_QE + MT * 64;            // [RING] exponent of the slot's tile
+    static constexpr int OFF_BAR = OFF_META + RING * 4;          // full[RING], empty[RING], abort
+    static constexpr int SMEM = OFF_BAR + 2 * RING * 8 + 16;
+    static_assert(OFF_BAR % 8 == 0 && SMEM <= 232448, "exceeds the 227 KB a CTA may use");
+    static_assert(AT_WARPS * 16384 <= RING * ENTRY, "the warps' sums do not fit the ring");
+};
+
+struct Where { int s, h, t; };                       // sequence, kv head, tile of the group
+
+__host__ __device__ __forceinline__ int share_lo(const Kv8AttnParams &p, int cta) {
+    return (int)((int64_t)p.total_tiles * cta / p.n_cta);
+}
+// The CTA whose share holds tile T: the largest c with floor(total * c / n) <= T.
+__host__ __device__ __forceinline__ int share_of(const Kv8AttnParams &p, int T) {
+    return (int)((((int64_t)T + 1) * p.n_cta - 1) / p.total_tiles);
+}
+__device__ __forceinline__ Where locate(const Kv8AttnParams &p, int T) {
+    int s = 0, e = p.n_seq - 1;
+    while (s < e) {
+        const int m = (s + e + 1) >> 1;
+        if (p.seq[m].cum_tiles <= T) s = m; else e = m - 1;
+    }
+    const int rel = T - p.seq[s].cum_tiles, n = p.seq[s].n_tiles;
+    Where w;
+    w.s = s; w.h = rel / n; w.t = rel - w.h * n;
+    return w;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void bar_all() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__device__ __forceinline__ float load1(const void *g, size_t i, int io) {
+    return io == DT_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(g)[i]) : reinterpret_cast<const float *>(g)[i];
+}
+// Four finished dims of one row: divided by the denominator already; gated and stored.
+__device__ __forceinline__ void store_out(const Kv8AttnParams &p, const Kv8AttnSeq &sq, size_t rh, int d4, float4 o) {
+    if (sq.gate) {
+        const size_t gi = rh * p.gate_stride + d4;
+        o.x /= 1.0f + __expf(-load1(sq.gate, gi, p.io)); o.y /= 1.0f + __expf(-load1(sq.gate, gi + 1, p.io));
+        o.z /= 1.0f + __expf(-load1(sq.gate, gi + 2, p.io)); o.w /= 1.0f + __expf(-load1(sq.gate, gi + 3, p.io));
+    }
+    if (p.io == DT_BF16)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(sq.out) + rh * 256 + d4) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+    else
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(sq.out) + rh * 256 + d4) = o;
+}
+
+template <int MT, bool F32>
+__global__ void __launch_bounds__(AT_THREADS, 1) kv8_attn_kernel(const __grid_constant__ Kv8AttnParams p) {
+    using Cfg = AtCfg<MT>;
+    constexpr int KG = Cfg::KG, NS = Cfg::NS, LAG = Cfg::LAG;
+    constexpr int RT = F32 ? 8 : 16;                 // query rows of a row tile
+    extern __shared__ __align__(1024) uint8_t smem[];
+    float *sm_m = reinterpret_cast<float *>(smem + Cfg::OFF_M);
+    float *sm_l = reinterpret_cast<float *>(smem + Cfg::OFF_L);
+    int *sm_qe = reinterpret_cast<int *>(smem + Cfg::OFF_QE);
+    int *meta = reinterpret_cast<int *>(smem + Cfg::OFF_META);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::OFF_BAR);
+    uint64_t *empty = full + RING;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(empty + RING);
+
+    if (smem_u32(smem) & 1023u) {                    // swizzled boxes need 1024-byte alignment
+        if (threadIdx.x == 0) report(p.status, QW_ST_BAD_SMEM);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int mt = warp % MT, kg = warp / MT;
+    const int g = lane >> 2, t = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], MT); }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_next();
+
+    uint8_t *ring = smem + kg * NS * ENTRY;
+    full += kg * NS; empty += kg * NS; meta += kg * NS;
+    const int lo = share_lo(p, blockIdx.x), hi = share_lo(p, blockIdx.x + 1);
+    Where w = locate(p, lo);
+    uint32_t E0 = 0;                                 // ring entries of this kg group before the current segment
+
+    for (int T = lo; T < hi;) {
+        const Kv8AttnSeq &sq = p.seq[w.s];
+        const int seg_t0 = w.t, seg_n = min(sq.n_tiles - w.t, hi - T);
+        const int valid = sq.rows * p.gqa, head0 = w.h * p.gqa;
+        const int n_keys = sq.base_pos + sq.rows;
+        const int nt = kg < seg_n ? (seg_n - kg + KG - 1) / KG : 0;      // this warp's tiles
+        const uint32_t E1 = E0 + 2 * nt;
+
+        // ---- loads: entry E of the group is K (even) or V (odd) of its tile (E - E0) / 2 ----
+        int win_k = 0, win_v = 0, win_e = 0;         // code rows and exponents of 32 tiles, one per lane
+        auto window = [&](int i0) {
+            const int i = i0 + lane;
+            if (i < nt) {
+                const int key = (seg_t0 + kg + i * KG) * TILE;
+                const int64_t kr = code_row(sq.kc, w.h, key), vr = code_row(sq.vc, w.h, key);
+                if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
+                win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
+                const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key / BLK]);
+                const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key / BLK]);
+                win_e = (ek & 0xffff) | (ev << 16);
+            }
+        };
+        auto load = [&](uint32_t E) {                // the whole warp mt == 0
+            const int i = (int)(E - E0) >> 1, is_v = (int)(E - E0) & 1;
+            if (!is_v && (i & 31) == 0) window(i);
+            const int row = __shfl_sync(0xffffffffu, is_v ? win_v : win_k, i & 31);
+            const int ex = __shfl_sync(0xffffffffu, win_e, i & 31);
+            if (lane == 0) {
+                const uint32_t slot = E % NS;
+                if (MT > 1 && E >= NS) mbar_wait(&empty[slot], (E / NS - 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
+                meta[slot] = is_v ? ex >> 16 : (int)(int16_t)(ex & 0xffff);
+                mbar_expect_tx(&full[slot], ENTRY);
+                const CUtensorMap *map = &p.maps[is_v ? sq.vmap : sq.kmap];
+                tma_load_2d(ring + slot * ENTRY, map, 0, row, &full[slot]);
+                tma_load_2d(ring + slot * ENTRY + BOX, map, 128, row, &full[slot]);
+            }
+            __syncwarp();
+        };
+        // a finished entry's slot is handed back; the loader refills the slot that fell free LAG entries ago
+        auto done = [&](uint32_t E) {
+            __syncwarp();
+            if (MT > 1 && lane == 0) mbar_arrive(&empty[E % NS]);
+            if (mt == 0) {
+                const uint32_t nx = E + NS - LAG;
+                if (E >= E0 + LAG && nx < E1) load(nx);
+            }
+        };
+        if (mt == 0)
+            for (uint32_t E = E0; E < E1 && E < E0 + NS; E++) load(E);
+
+        // ---- Q: one warp per row, 8 dims per lane, scaled to [2^13, 2^14) and put where the tensor op's A fragments
+        // are read: step 4 q + i of a row tile takes dims 64 q + 16 t + 4 i + {0, 1 | 2, 3} of lane (g, t) ----
+        for (int row = warp; row < MT * RT; row += AT_WARPS) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = 0.0f;
+            if (row < valid) {
+                const int r = row / p.gqa, hh = row - r * p.gqa;
+                const size_t at = ((size_t)r * p.q_heads + head0 + hh) * 256 + lane * 8;
+                if constexpr (F32) {
+                    const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at);
+                    const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at + 4);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                } else {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(sq.q) + at);
+                    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
+                }
+            }
+            float mx = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
+            mx = warp_max(mx);
+            // row exponent: x * 2^-qe is below 2^14 (kept where 2^-qe and 2^qe are normal numbers)
+            const int qe = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 13, -100), 100);
+            const float f = pow2f(-qe);
+            if (lane == 0) sm_qe[row] = qe;
+            const int q = lane >> 3, tt = (lane >> 1) & 3, i0 = (lane & 1) * 2;
+            const int tile = row / RT, rr = row % RT;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint32_t *fr = reinterpret_cast<uint32_t *>(smem + OFF_Q) + (((size_t)tile * 16 + q * 4 + i0 + i) * 32 + (rr & 7) * 4 + tt) * 4;
+                const float a = x[4 * i] * f, b = x[4 * i + 1] * f, c = x[4 * i + 2] * f, d = x[4 * i + 3] * f;
+                const uint32_t ab = pack_f16(a, b), cd = pack_f16(c, d);
+                if constexpr (F32) {
+                    const float2 hab = h2f2(ab), hcd = h2f2(cd);
+                    *reinterpret_cast<uint4 *>(fr) = make_uint4(ab, pack_f16(a - hab.x, b - hab.y), cd, pack_f16(c - hcd.x, d - hcd.y));
+                } else {
+                    fr[rr >> 3] = ab; fr[2 + (rr >> 3)] = cd;
+                }
+            }
+        }
+        bar_all();
+
+        float o[32][4];
+#pragma unroll
+        for (int n = 0; n < 32; n++) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        const int row0 = mt * RT + g, row1 = row0 + 8;                   // (f32: only row0, its low part in tensor row 8 + g)
+        const int lim0 = row0 < valid ? sq.base_pos + row0 / p.gqa : n_keys - 1;
+        const int lim1 = F32 ? lim0 : row1 < valid ? sq.base_pos + row1 / p.gqa : n_keys - 1;
+        const float sc0 = p.scale * LOG2E * pow2f(sm_qe[row0]);
+        const float sc1 = F32 ? sc0 : p.scale * LOG2E * pow2f(sm_qe[row1]);
+        const uint32_t q_base = smem_u32(smem + OFF_Q) + mt * 8192 + lane * 16;
+
+        for (int i = 0; i < nt; i++) {
+            const int key0 = (seg_t0 + kg + i * KG) * TILE;
+            const uint32_t EK = E0 + 2 * i, EV = EK + 1;
+            // ---- S = Q K^T: column n of the tensor op is token n ^ 4 (n & 1) of its group of eight, so that the eight
+            // lanes of a shared-memory phase meet eight different bank groups ----
+            float s[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            mbar_wait(&full[EK % NS], (EK / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            const int ek = meta[EK % NS];
+            {
+                const uint32_t tok = (uint32_t)(g ^ ((g & 1) << 2));
+                const uint32_t kb = smem_u32(ring + (EK % NS) * ENTRY) + tok * 128;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t kw[4][4];
+#pragma unroll
+                    for (int n = 0; n < 4; n++)
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(kw[n][0]), "=r"(kw[n][1]), "=r"(kw[n][2]), "=r"(kw[n][3])
+                                     : "r"(kb + (q >> 1) * BOX + n * 1024 + ((((uint32_t)(4 * (q & 1) + t)) ^ tok) << 4)));
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t a0, a1, a2, a3;
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3) : "r"(q_base + (q * 4 + k) * 512));
+#pragma unroll
+                        for (int n = 0; n < 4; n++) mma_f16(s[n], a0, a1, a2, a3, f16x2_lo(kw[n][k]), f16x2_hi(kw[n][k]));
+                    }
+                }
+            }
+            done(EK);
+            mbar_wait(&full[EV % NS], (EV / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            const int ev = meta[EV % NS];
+
+            // ---- online softmax ----
+            const float k0 = sc0 * pow2f(ek), k1 = sc1 * pow2f(ek), fv = (float)ev;
+            if constexpr (F32) {
+#pragma unroll
+                for (int n = 0; n < 4; n++) { s[n][0] += s[n][2]; s[n][1] += s[n][3]; }
+            }
+            constexpr int ROWS = F32 ? 2 : 4;         // values of a thread: two columns of one or two rows
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int c = 0; c < ROWS; c++) s[n][c] = fmaf(s[n][c], c < 2 ? k0 : k1, fv);
+            if (key0 + TILE > sq.base_pos + 1) {
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int c = 0; c < ROWS; c++) {
+                        const int key = key0 + n * 8 + ((c & 1) ? ((2 * t + 1) ^ 4) : 2 * t);
+                        if (key > (c < 2 ? lim0 : lim1)) s[n][c] = -INFINITY;
+                    }
+            }
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
+                if (!F32) x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
+            }
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+            if (!F32) {
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+            }
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                const float f0 = m0 == n0 ? 1.0f : ex2(m0 - n0), f1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
+                l0 *= f0; l1 *= f1;
+#pragma unroll
+                for (int n = 0; n < 32; n++) { o[n][0] *= f0; o[n][1] *= f0; o[n][2] *= F32 ? f0 : f1; o[n][3] *= F32 ? f0 : f1; }
+                m0 = n0; m1 = n1;
+            }
+            const float b0 = (m0 == -INFINITY ? 0.0f : m0) - W_SHIFT, b1 = (m1 == -INFINITY ? 0.0f : m1) - W_SHIFT;
+            uint32_t pa[2][4];
+            float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const float w0 = ex2(s[n][0] - b0), w1 = ex2(s[n][1] - b0);
+                a0 += w0 + w1;
+                const uint32_t hi = pack_f16(w0, w1);
+                pa[n >> 1][(n & 1) * 2] = hi;
+                if constexpr (F32) {
+                    const float2 h = h2f2(hi);
+                    pa[n >> 1][(n & 1) * 2 + 1] = pack_f16(w0 - h.x, w1 - h.y);
+                } else {
+                    const float w2 = ex2(s[n][2] - b1), w3 = ex2(s[n][3] - b1);
+                    a1 += w2 + w3;
+                    pa[n >> 1][(n & 1) * 2 + 1] = pack_f16(w2, w3);
+                }
+            }
+            const float iv = pow2f(-ev);
+            l0 = fmaf(a0, iv, l0); l1 = fmaf(a1, iv, l1);
+
+            // ---- O += W V: column g of tile (x, d) is dim 128 x + 16 g + d; the two tokens of a B register are
+            // interleaved byte by byte before they are widened ----
+            const uint32_t vb = smem_u32(ring + (EV % NS) * ENTRY);
+            const bool ragged = key0 + TILE > n_keys;     // rows past the last key may hold anything
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+                const uint32_t ta = 16 * kk + 2 * t, tb = 16 * kk + ((2 * t + 1) ^ 4);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    uint32_t v[4][4];                     // tokens ta, tb, ta + 8, tb + 8
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t tok = ((c & 1) ? tb : ta) + (c >> 1) * 8;
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[c][0]), "=r"(v[c][1]), "=r"(v[c][2]), "=r"(v[c][3])
+                                     : "r"(vb + x * BOX + tok * 128 + (((uint32_t)g ^ (tok & 7)) << 4)));
+                        if (ragged && key0 + (int)tok >= n_keys) v[c][0] = v[c][1] = v[c][2] = v[c][3] = 0;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140), p1 = __byte_perm(v[0][k], v[1][k], 0x7362);
+                        const uint32_t r0 = __byte_perm(v[2][k], v[3][k], 0x5140), r1 = __byte_perm(v[2][k], v[3][k], 0x7362);
+                        const int n = x * 16 + k * 4;
+                        mma_f16(o[n], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_lo(p0), f16x2_lo(r0));
+                        mma_f16(o[n + 1], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_hi(p0), f16x2_hi(r0));
+                        mma_f16(o[n + 2], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_lo(p1), f16x2_lo(r1));
+                        mma_f16(o[n + 3], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_hi(p1), f16x2_hi(r1));
+                    }
+                }
+            }
+            done(EV);
+        }
+        E0 = E1;
+
+        // ---- segment end: the KG warps of a row tile put their sums side by side into the ring (idle: every entry
+        // was consumed), and all threads add them up ----
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        if (t == 0) {
+            sm_m[kg * MT * RT + row0] = m0; sm_l[kg * MT * RT + row0] = l0;
+            if (!F32) { sm_m[kg * MT * RT + row1] = m1; sm_l[kg * MT * RT + row1] = l1; }
+        }
+        bar_all();
+        float M0 = -INFINITY, M1 = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KG; k++) {
+            M0 = fmaxf(M0, sm_m[k * MT * RT + row0]);
+            if (!F32) M1 = fmaxf(M1, sm_m[k * MT * RT + row1]);
+        }
+        {
+            const float f0 = m0 == M0 ? 1.0f : ex2(m0 - M0), f1 = m1 == M1 ? 1.0f : ex2(m1 - M1);
+            // the thread's dims of a row: 128 x + 32 t + [0, 16) and + [16, 32), as 16-byte pieces; piece c of a row
+            // sits at c ^ (t + 4 (row & 1)), which spreads a phase's eight lanes over the banks
+            float *own = reinterpret_cast<float *>(smem) + (size_t)warp * 4096;
+            const uint32_t sw = (uint32_t)(t + ((g & 1) << 2));
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        const int n = x * 16 + d * 4;
+                        const uint32_t piece = ((uint32_t)(x * 32 + t * 8 + c * 4 + d)) ^ sw;
+                        float4 a = make_float4(o[n][c], o[n + 1][c], o[n + 2][c], o[n + 3][c]);
+                        const float4 b = make_float4(o[n][2 + c], o[n + 1][2 + c], o[n + 2][2 + c], o[n + 3][2 + c]);
+                        if constexpr (F32) {
+                            a = make_float4((a.x + b.x) * f0, (a.y + b.y) * f0, (a.z + b.z) * f0, (a.w + b.w) * f0);
+                            *reinterpret_cast<float4 *>(own + g * 256 + piece * 4) = a;
+                        } else {
+                            *reinterpret_cast<float4 *>(own + g * 256 + piece * 4) = make_float4(a.x * f0, a.y * f0, a.z * f0, a.w * f0);
+                            *reinterpret_cast<float4 *>(own + (g + 8) * 256 + piece * 4) = make_float4(b.x * f1, b.y * f1, b.z * f1, b.w * f1);
+                        }
+                    }
+        }
+        bar_all();
+        const bool whole = seg_t0 == 0 && seg_n == sq.n_tiles;
+        const size_t slot = (size_t)blockIdx.x + (size_t)w.s * p.kv_heads + w.h;
+        for (int idx = threadIdx.x; idx < valid * 64; idx += AT_THREADS) {
+            const int row = idx >> 6, pc = idx & 63;
+            const int tile = row / RT, rr = row % RT;
+            const uint32_t piece = (uint32_t)pc ^ (uint32_t)(((pc >> 3) & 3) + ((rr & 1) << 2));
+            float M = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < KG; k++) M = fmaxf(M, sm_m[k * MT * RT + row]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KG; k++) {
+                const float mk = sm_m[k * MT * RT + row];
+                L += sm_l[k * MT * RT + row] * (mk == M ? 1.0f : ex2(mk - M));
+                const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + (size_t)(k * MT + tile) * 4096 + rr * 256 + piece * 4);
+                acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
+            }
+            if (whole) {
+                const int r = row / p.gqa;
+                const size_t rh = (size_t)r * p.q_heads + head0 + (row - r * p.gqa);
+                const float inv = 1.0f / L;
+                store_out(p, sq, rh, pc * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+            } else {
+                const size_t pi = slot * p.slot_rows + row;
+                *reinterpret_cast<float4 *>(p.pacc + pi * 256 + pc * 4) = acc;
+                if (pc == 0) *reinterpret_cast<float2 *>(p.pstat + pi * 2) = make_float2(M, L);
+            }
+        }
+        T += seg_n;
+        w.t = 0;                                          // the next segment, if any, begins the next group
+        if (++w.h == p.kv_heads) { w.h = 0; w.s++; }
+        fence_proxy_async();                              // the ring goes back to the copy engine
+        bar_all();
+    }
+    if (*abort_flag)                                      // a wait gave up: copies of this CTA may still be under way
+        for (int i = 0; i < 4096; i++) __nanosleep(10000);
+}
+
+// Partials of a cut group: one block per (group, row); the four quarters of the block take every fourth partial.
+__global__ void __launch_bounds__(256) kv8_merge_kernel(const __grid_constant__ Kv8AttnParams p, int max_valid) {
+    __shared__ float w_s[256];
+    __shared__ float red_s[2][8];
+    __shared__ __align__(16) float acc_s[3][256];
+    pdl_launch_next();
+    pdl_wait();
+    const int gi = blockIdx.x / max_valid, row = blockIdx.x - gi * max_valid;
+    const int s = gi / p.kv_heads, h = gi - s * p.kv_heads;
+    const Kv8AttnSeq &sq = p.seq[s];
+    if (row >= sq.rows * p.gqa) return;
+    const int G0 = sq.cum_tiles + h * sq.n_tiles, c0 = share_of(p, G0), parts = share_of(p, G0 + sq.n_tiles - 1) - c0 + 1;
+    if (parts == 1) return;                               // written whole
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const size_t pi0 = (size_t)(c0 + gi) * p.slot_rows + row;
+    float mq = -INFINITY, lq = 0.0f;
+    if (tid < parts) {
+        const float2 st = *reinterpret_cast<const float2 *>(p.pstat + (pi0 + (size_t)tid * p.slot_rows) * 2);
+        mq = st.x; lq = st.y;
+    }
+    float m = warp_max(mq);
+    if (lane == 0) red_s[0][warp] = m;
+    __syncthreads();
+    m = red_s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) m = fmaxf(m, red_s[0][i]);
+    const float wq = mq == m ? 1.0f : ex2(mq - m);
+    w_s[tid] = wq;
+    const float d = warp_sum(tid < parts ? lq * wq : 0.0f);
+    if (lane == 0) red_s[1][warp] = d;
+    __syncthreads();
+    float den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) den += red_s[1][i];
+    const int quarter = tid >> 6, d4 = (tid & 63) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = quarter; q < parts; q += 4) {
+        const float4 a = *reinterpret_cast<const float4 *>(p.pacc + (pi0 + (size_t)q * p.slot_rows) * 256 + d4);
+        const float f = w_s[q];
+        acc.x += a.x * f; acc.y += a.y * f; acc.z += a.z * f; acc.w += a.w * f;
+    }
+    if (quarter > 0) *reinterpret_cast<float4 *>(&acc_s[quarter - 1][d4]) = acc;
+    __syncthreads();
+    if (quarter > 0) return;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        const float4 a = *reinterpret_cast<const float4 *>(&acc_s[i][d4]);
+        acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
+    }
+    const int r = row / p.gqa;
+    const float inv = 1.0f / den;
+    store_out(p, sq, (size_t)r * p.q_heads + h * p.gqa + (row - r * p.gqa), d4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+}
+
+void pdl_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &attr, dim3 grid, unsigned block, size_t smem, cudaStream_t s) {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg = cudaLaunchConfig_t();
+    cfg.gridDim = grid; cfg.blockDim = dim3(block); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.attrs = &attr; cfg.numAttrs = g_tune_pdl ? 1 : 0;
+}
+
+template <int MT, bool F32>
+void launch_attn_t(cudaStream_t s, const Kv8AttnParams &p) {
+    static bool configured[64] = {false};      // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !configured[dev]) {
+        cudaFuncSetAttribute(kv8_attn_kernel<MT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, AtCfg<MT>::SMEM);
+        configured[dev] = true;
+    }
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(cfg, attr, dim3((unsigned)p.n_cta), AT_THREADS, AtCfg<MT>::SMEM, s);
+    cudaLaunchKernelEx(&cfg, kv8_attn_kernel<MT, F32>, p);
+    g_launches++;
+}
+
+}  // namespace
+
+void launch_kv8_write(cudaStream_t s, const Kv8WriteParams &p) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(cfg, attr, dim3((unsigned)p.max_blocks, (unsigned)p.kv_heads * 2, (unsigned)p.n_seq), WR_THREADS, 0, s);
+    if (p.io == DT_BF16) cudaLaunchKernelEx(&cfg, kv8_write_kernel<__nv_bfloat16>, p);
+    else cudaLaunchKernelEx(&cfg, kv8_write_kernel<float>, p);
+    g_launches++;
+}
+
+void launch_kv8_read(cudaStream_t s, void *dst, int io, const Kv8Layer &c, int kv_heads, int pos0, int n) {
+    constexpr int rows = RD_THREADS / 32 * RD_ROWS;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(cfg, attr, dim3((unsigned)((n + rows - 1) / rows), (unsigned)kv_heads), RD_THREADS, 0, s);
+    if (io == DT_BF16) cudaLaunchKernelEx(&cfg, kv8_read_kernel<__nv_bfloat16>, reinterpret_cast<__nv_bfloat16 *>(dst), c, pos0, n);
+    else cudaLaunchKernelEx(&cfg, kv8_read_kernel<float>, reinterpret_cast<float *>(dst), c, pos0, n);
+    g_launches++;
+}
+
+void kv8_attn_plan(Kv8AttnParams &p) {
+    int cum = 0, valid = 0;
+    for (int i = 0; i < p.n_seq; i++) {
+        Kv8AttnSeq &s = p.seq[i];
+        s.n_tiles = (s.base_pos + s.rows + TILE - 1) / TILE;
+        s.cum_tiles = cum;
+        cum += s.n_tiles * p.kv_heads;
+        valid = std::max(valid, s.rows * p.gqa);
+    }
+    p.total_tiles = cum;
+    p.n_cta = std::min(std::min(sm_count(), 256), cum);      // the merge reads one partial per thread of 256
+    p.slot_rows = valid;
+}
+
+size_t kv8_attn_scratch_bytes(const Kv8AttnParams &p) {
+    return ((size_t)p.n_cta + (size_t)p.n_seq * p.kv_heads) * p.slot_rows * 258 * sizeof(float);
+}
+
+void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scratch) {
+    const size_t slots = (size_t)p.n_cta + (size_t)p.n_seq * p.kv_heads;
+    p.pacc = reinterpret_cast<float *>(scratch);
+    p.pstat = p.pacc + slots * p.slot_rows * 256;
+    const int valid = max_rows * p.gqa, f32 = p.io == DT_F32, per = f32 ? 8 : 16;
+    const int mt = (valid + per - 1) / per;
+    if (f32) { if (mt <= 1) launch_attn_t<1, true>(s, p); else if (mt <= 2) launch_attn_t<2, true>(s, p); else launch_attn_t<4, true>(s, p); }
+    else { if (mt <= 1) launch_attn_t<1, false>(s, p); else if (mt <= 2) launch_attn_t<2, false>(s, p); else launch_attn_t<4, false>(s, p); }
+    bool cut = false;
+    for (int i = 0; i < p.n_seq && !cut; i++)
+        for (int h = 0; h < p.kv_heads && !cut; h++) {
+            const int g0 = p.seq[i].cum_tiles + h * p.seq[i].n_tiles;
+            cut = share_of(p, g0) != share_of(p, g0 + p.seq[i].n_tiles - 1);
+        }
+    if (!cut) return;                          // every group was written whole
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(cfg, attr, dim3((unsigned)(p.n_seq * p.kv_heads * valid)), 256, 0, s);
+    cudaLaunchKernelEx(&cfg, kv8_merge_kernel, p, valid);
+    g_launches++;
+}
+
+}  // namespace qw

@@ -8,7 +8,7 @@
 // "encoding nothing", device errors surface as a string from qw_cmd_error after
 // qw_cmd_wait.  There is no CPU path: without a CUDA device qw_gpu_init fails
 // and every op declines.
-#include "../../include/qwasar_cuda.h"
+#include "../../include/qwasar_kv8.h"
 #include "qw_kernels.h"
 
 #include <algorithm>
@@ -182,6 +182,7 @@ const char *status_text(int code) {
         case QW_ST_BAD_PAGE: return "attention reached a cache position whose page was never mapped";
         case QW_ST_BAD_SMEM: return "the prefill kernel's shared-memory window was not 1024-byte aligned";
         case QW_ST_PEER_TIMEOUT: return "the partial of another GPU did not arrive within the exchange's time limit";
+        case QW_ST_KV8_NONFINITE: return "a key or value written to an 8-bit cache was NaN or infinite";
         default: return "unknown kernel status";
     }
 }
@@ -209,11 +210,15 @@ struct Pool {
     int refs;                             // arenas (and the pool's own handle) that keep it alive
     CUtensorMap map;                      // 32-row boxes (split-KV kernel)
     CUtensorMap map64;                    // 64-row boxes (prefill kernel)
+    CUtensorMap map8;                     // the same range as 256-byte rows of 8-bit codes, boxes of 128 bytes x 32 rows
 };
 struct Arena {
     Pool *pool;
     int n_layers, kv_heads, max_ctx, head_dim;
+    int elem_bytes;                       // 2: bf16 rows; 1: e4m3 codes (an 8-bit arena)
+    int page_tokens;                      // tokens per 32 KB page: 64 or 128
     int pages_per_head;
+    uint8_t *exps_dev = nullptr;          // 8-bit arenas: [n_layers, kv_heads, blocks of 64 tokens] exponent bytes
     int64_t max_pages;
     std::vector<int32_t> table_host;      // [n_layers, kv_heads, pages_per_head], -1 = unmapped
     int32_t *table_dev;
@@ -228,6 +233,18 @@ bool encode_rows_map(CUtensorMap *m, void *base, uint64_t rows, uint32_t box_row
     CUresult r = G.encodeTiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed (%d)", (int)r); return false; }
+    return true;
+}
+
+// Rows of 256 one-byte codes, as boxes of 128 codes x 32 rows.
+bool encode_codes_map(CUtensorMap *m, void *base, uint64_t rows) {
+    cuuint64_t dims[2] = {QW_HEAD_DIM, rows};
+    cuuint64_t strides[1] = {QW_HEAD_DIM};
+    cuuint32_t box[2] = {128, 32};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = G.encodeTiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed (%d)", (int)r); return false; }
     return true;
 }
@@ -311,8 +328,8 @@ bool pool_grow(Pool *a) {
 // page-table entries to the device in stream order.  Pages below first_token are left alone: a
 // rank that owns only a range of positions maps only that range.
 bool arena_ensure(Arena *a, int layer, int first_token, int n_tokens, cudaStream_t stream) {
-    const int need = (n_tokens + QW_PAGE_TOKENS - 1) / QW_PAGE_TOKENS;
-    const int first_page = std::max(first_token, 0) / QW_PAGE_TOKENS;
+    const int need = (n_tokens + a->page_tokens - 1) / a->page_tokens;
+    const int first_page = std::max(first_token, 0) / a->page_tokens;
     if (need > a->pages_per_head) { set_error("arena: %d tokens exceed max_ctx %d", n_tokens, a->max_ctx); return false; }
     Pool *pl = a->pool;
     for (int h = 0; h < a->kv_heads; h++) {
@@ -386,7 +403,8 @@ Pool *pool_create(size_t max_bytes, uint32_t shuffle) {
     }
     // the tensor maps span the whole reserved range; rows of unmapped pages are never addressed
     if (!encode_rows_map(&pl->map, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 512), 32) ||
-        !encode_rows_map(&pl->map64, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 512), 64)) { pool_release(pl); return nullptr; }
+        !encode_rows_map(&pl->map64, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 512), 64) ||
+        !encode_codes_map(&pl->map8, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 256))) { pool_release(pl); return nullptr; }
     return pl;
 }
 
@@ -398,6 +416,7 @@ void arena_destroy(Arena *a) {
     // recycled page owns every row of it only after it has appended that row)
     for (int32_t id : a->table_host) if (id >= 0) a->pool->free_pages.push_back(id);
     if (a->table_dev) cudaFree(a->table_dev);
+    if (a->exps_dev) cudaFree(a->exps_dev);
     pool_release(a->pool);
     delete a;
 }
@@ -460,6 +479,13 @@ void *dev_range(qw_cmd c, qw_ref r, size_t bytes, bool write, size_t align = 16)
     return (char *)b->dev + r.off;
 }
 
+// Whether the command buffer's stream is being captured into a graph: nothing may be allocated, and no page mapped, then.
+bool capturing(qw_cmd c) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c->stream, &st) != cudaSuccess) { cudaGetLastError(); return false; }
+    return st != cudaStreamCaptureStatusNone;
+}
+
 void *cmd_scratch(qw_cmd c, size_t bytes) {
     bytes = (bytes + 1023) & ~(size_t)1023;
     if (!c->scratch.empty() && c->scratch.back().n >= bytes) return c->scratch.back().p;
@@ -474,6 +500,7 @@ void *cmd_scratch(qw_cmd c, size_t bytes) {
         G.scratch_pool.erase(G.scratch_pool.begin() + (long)best);
     } else {
         s.n = std::max(bytes, (size_t)8 << 20);
+        if (capturing(c)) { cmd_fail(c, "this op needs %zu bytes of scratch the command buffer does not hold yet: encode it once before the capture", bytes); return nullptr; }
         if (cudaMalloc(&s.p, s.n) != cudaSuccess) { cmd_fail(c, "cannot allocate %zu bytes of scratch", s.n); return nullptr; }
     }
     c->scratch.push_back(s);
@@ -496,6 +523,7 @@ bool resolve_cache(qw_cmd c, qw_ref ref, int32_t kv_heads, int32_t max_ctx, int3
     const size_t layer_bytes = (size_t)kv_heads * max_ctx * head_dim * 2;
     if (b->kind == BUF_ARENA) {
         Arena *a = b->arena;
+        if (a->elem_bytes != 2) { cmd_fail(c, "an 8-bit arena is a cache operand of the kv8 ops only"); return false; }
         if (a->kv_heads != kv_heads || a->max_ctx != max_ctx || a->head_dim != head_dim) {
             cmd_fail(c, "arena was created for [%d heads, %d ctx, %d dim], op says [%d, %d, %d]", a->kv_heads, a->max_ctx,
                      a->head_dim, kv_heads, max_ctx, head_dim);
@@ -533,6 +561,73 @@ bool resolve_cache(qw_cmd c, qw_ref ref, int32_t kv_heads, int32_t max_ctx, int3
         if (map_rows) *map_rows = (int64_t)rows;
     }
     return true;
+}
+
+// ---- 8-bit caches ----
+size_t kv8_blocks(int32_t max_ctx) { return ((size_t)max_ctx + QW_KV8_BLOCK - 1) / QW_KV8_BLOCK; }
+size_t kv8_layer_bytes(int32_t kv_heads, int32_t max_ctx) {
+    return ((size_t)kv_heads * max_ctx * QW_HEAD_DIM + (size_t)kv_heads * kv8_blocks(max_ctx) + 255) & ~(size_t)255;
+}
+
+// One layer of an 8-bit cache -> Kv8Layer + tensor map; `append`: the pages of [first_token, n_tokens) are mapped.
+bool resolve_kv8(qw_cmd c, qw_ref ref, int32_t kv_heads, int32_t max_ctx, int32_t first_token, int32_t n_tokens, bool append,
+                 Kv8Layer *out, CUtensorMap *map) {
+    qw_buf b = ref.buf;
+    if (!b) { cmd_fail(c, "cache operand is null"); return false; }
+    if (b->kind == BUF_POOL) { cmd_fail(c, "a page pool is not a cache: allocate an arena in it"); return false; }
+    if (b->device != c->device) { cmd_fail(c, "cache operand lives on device %d, the command buffer on %d", b->device, c->device); return false; }
+    const size_t layer_bytes = kv8_layer_bytes(kv_heads, max_ctx);
+    out->max_ctx = max_ctx;
+    out->exp_stride = (int32_t)kv8_blocks(max_ctx);
+    if (b->kind == BUF_ARENA) {
+        Arena *a = b->arena;
+        if (a->elem_bytes != 1) { cmd_fail(c, "a bf16 arena is not an 8-bit cache"); return false; }
+        if (a->kv_heads != kv_heads || a->max_ctx != max_ctx) {
+            cmd_fail(c, "arena was created for [%d heads, %d ctx], op says [%d, %d]", a->kv_heads, a->max_ctx, kv_heads, max_ctx);
+            return false;
+        }
+        if (ref.off % layer_bytes || ref.off / layer_bytes >= (size_t)a->n_layers) { cmd_fail(c, "arena offset %zu is not a layer of it", ref.off); return false; }
+        const int layer = (int)(ref.off / layer_bytes);
+        if (append) {
+            if (capturing(c)) {
+                const int32_t *tab = a->table_host.data() + (size_t)layer * kv_heads * a->pages_per_head;
+                for (int h = 0; h < kv_heads; h++)
+                    for (int pg = first_token / a->page_tokens; pg * (int64_t)a->page_tokens < n_tokens; pg++)
+                        if (tab[(size_t)h * a->pages_per_head + pg] < 0) { cmd_fail(c, "an append into pages that are not mapped yet cannot be captured"); return false; }
+            } else if (!arena_ensure(a, layer, first_token, n_tokens, c->stream)) { cmd_fail(c, "%s", SH.last_error); return false; }
+        }
+        out->base = reinterpret_cast<uint8_t *>(a->pool->va);
+        out->table = a->table_dev + (size_t)layer * kv_heads * a->pages_per_head;
+        out->pt_stride = a->pages_per_head;
+        out->exps = a->exps_dev + (size_t)layer * kv_heads * out->exp_stride;
+        if (map) *map = a->pool->map8;
+        return true;
+    }
+    uint8_t *d = (uint8_t *)dev_range(c, ref, layer_bytes, append, 128);
+    if (!d) return false;
+    out->base = d;
+    out->table = nullptr;
+    out->pt_stride = 0;
+    out->exps = d + (size_t)kv_heads * max_ctx * QW_HEAD_DIM;
+    if (map) {
+        const uint64_t rows = (uint64_t)kv_heads * max_ctx;
+        const auto key = std::make_pair((uintptr_t)d, rows | (uint64_t)1 << 63);      // (bf16 maps: rows * 128 + box rows)
+        auto it = G.map_cache.find(key);
+        if (it == G.map_cache.end()) {
+            CUtensorMap m;
+            if (!encode_codes_map(&m, d, rows)) { cmd_fail(c, "%s", SH.last_error); return false; }
+            it = G.map_cache.emplace(key, m).first;
+        }
+        *map = it->second;
+    }
+    return true;
+}
+// dev_range for operands that must live on the command buffer's device.
+void *near_range(qw_cmd c, qw_ref r, size_t bytes, bool write, size_t align = 16) {
+    if (!r.buf) { cmd_fail(c, "an operand is null"); return nullptr; }
+    if (r.buf->device != c->device) { cmd_fail(c, "operand lives on device %d, the command buffer on %d", r.buf->device, c->device); return nullptr; }
+    if (r.off > r.buf->len || bytes > r.buf->len) { cmd_fail(c, "operand [%zu, +%zu) exceeds its buffer (%zu bytes)", r.off, bytes, r.buf->len); return nullptr; }
+    return dev_range(c, r, bytes, write, align);
 }
 
 // Fills the schedule fields of a launch's sequences and sizes its grid.
@@ -629,6 +724,9 @@ struct SplitBatch {
 // With cs_table != nullptr, q_bf16 is instead the raw [rows, q_heads, 512] bf16 [q|gate] input: the kernel
 // norms (weights q_norm_w or nullptr, eps) and rotates its own query tiles, with the angles' cos / sin from
 // cs_table ([rows, 64] f32, left by the pre-op).
+bool run_prefill_on(qw_cmd c, PrefillParams &p, int64_t k_rows, int64_t v_rows, const __nv_bfloat16 *q_bf16, void *out, int out_dtype,
+                    const void *gate, int gate_dtype, int gate_stride, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t base_pos,
+                    float scale, const float *cs_table = nullptr, const uint16_t *q_norm_w = nullptr, float eps = 0.0f);
 bool run_prefill(qw_cmd c, const __nv_bfloat16 *q_bf16, void *out, int out_dtype, const void *gate, int gate_dtype,
                  int gate_stride, qw_ref kcache, qw_ref vcache, int32_t rows, int32_t q_heads, int32_t kv_heads,
                  int32_t max_ctx, int32_t base_pos, float scale, const float *cs_table = nullptr,
@@ -638,6 +736,13 @@ bool run_prefill(qw_cmd c, const __nv_bfloat16 *q_bf16, void *out, int out_dtype
     int64_t k_rows = 0, v_rows = 0;
     if (!resolve_cache(c, kcache, kv_heads, max_ctx, QW_HEAD_DIM, base_pos + rows, false, false, &p.kc, &p.kmap, 64, &k_rows)) return false;
     if (!resolve_cache(c, vcache, kv_heads, max_ctx, QW_HEAD_DIM, base_pos + rows, false, false, &p.vc, &p.vmap, 64, &v_rows)) return false;
+    return run_prefill_on(c, p, k_rows, v_rows, q_bf16, out, out_dtype, gate, gate_dtype, gate_stride, rows, q_heads, kv_heads, base_pos,
+                          scale, cs_table, q_norm_w, eps);
+}
+
+bool run_prefill_on(qw_cmd c, PrefillParams &p, int64_t k_rows, int64_t v_rows, const __nv_bfloat16 *q_bf16, void *out, int out_dtype,
+                    const void *gate, int gate_dtype, int gate_stride, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t base_pos,
+                    float scale, const float *cs_table, const uint16_t *q_norm_w, float eps) {
     p.q = q_bf16;
     p.out = out; p.out_dtype = out_dtype; p.gate = gate; p.gate_dtype = gate_dtype; p.gate_stride = gate_stride;
     p.rows = rows; p.base_pos = base_pos; p.q_heads = q_heads; p.kv_heads = kv_heads; p.gqa = q_heads / kv_heads;
@@ -932,11 +1037,13 @@ extern "C" bool qw_buf_download(qw_buf b, size_t off, void *dst, size_t len) {
 // arena API
 // ---------------------------------------------------------------------------------------
 static qw_buf arena_new(Pool *pool, bool private_pool, int32_t n_layers, int32_t kv_heads, int32_t max_ctx, int32_t head_dim,
-                        uint32_t shuffle_seed) {
+                        uint32_t shuffle_seed, int elem_bytes = 2) {
     if (n_layers <= 0 || kv_heads <= 0 || max_ctx <= 0 || head_dim != QW_HEAD_DIM) { set_error("arena: unsupported shape"); return nullptr; }
     Arena *a = new Arena();
     a->n_layers = n_layers; a->kv_heads = kv_heads; a->max_ctx = max_ctx; a->head_dim = head_dim;
-    a->pages_per_head = (max_ctx + QW_PAGE_TOKENS - 1) / QW_PAGE_TOKENS;
+    a->elem_bytes = elem_bytes;
+    a->page_tokens = elem_bytes == 1 ? QW_KV8_PAGE_TOKENS : QW_PAGE_TOKENS;
+    a->pages_per_head = (int)(((int64_t)max_ctx + a->page_tokens - 1) / a->page_tokens);
     a->max_pages = (int64_t)n_layers * kv_heads * a->pages_per_head;
     a->in_use = 0; a->table_dev = nullptr;
     if (private_pool) {
@@ -949,8 +1056,13 @@ static qw_buf arena_new(Pool *pool, bool private_pool, int32_t n_layers, int32_t
     a->table_host.assign((size_t)a->max_pages, -1);
     if (cudaMalloc(&a->table_dev, (size_t)a->max_pages * sizeof(int32_t)) != cudaSuccess) { set_error("arena: cannot allocate the page table"); arena_destroy(a); cudaGetLastError(); return nullptr; }
     cudaMemset(a->table_dev, 0xff, (size_t)a->max_pages * sizeof(int32_t));
+    if (elem_bytes == 1) {
+        const size_t n = (size_t)n_layers * kv_heads * kv8_blocks(max_ctx);
+        if (cudaMalloc(&a->exps_dev, n) != cudaSuccess) { set_error("arena: cannot allocate the exponents"); arena_destroy(a); cudaGetLastError(); return nullptr; }
+        cudaMemset(a->exps_dev, 0, n);
+    }
     cudaStreamSynchronize(0);   // the fill must not trail kernels launched on other streams
-    qw_buf b = new qw_buf_s{BUF_ARENA, (size_t)n_layers * kv_heads * max_ctx * head_dim * 2, nullptr,
+    qw_buf b = new qw_buf_s{BUF_ARENA, elem_bytes == 1 ? n_layers * kv8_layer_bytes(kv_heads, max_ctx) : (size_t)n_layers * kv_heads * max_ctx * head_dim * 2, nullptr,
                             reinterpret_cast<void *>(pool->va), false, false, false, a};
     b->device = G.device;
     return b;
@@ -978,6 +1090,19 @@ extern "C" qw_buf qw_kv_arena_alloc_in(qw_buf pool, int32_t n_layers, int32_t kv
     use_device(pool->device);
     return arena_new(pool->pool, false, n_layers, kv_heads, max_ctx, head_dim, 0);
 }
+extern "C" size_t qw_kv8_layer_bytes(int32_t kv_heads, int32_t max_ctx, int32_t head_dim) {
+    if (kv_heads <= 0 || max_ctx <= 0 || head_dim != QW_HEAD_DIM) return 0;
+    return kv8_layer_bytes(kv_heads, max_ctx);
+}
+extern "C" qw_buf qw_kv8_arena_alloc(int32_t n_layers, int32_t kv_heads, int32_t max_ctx, int32_t head_dim, uint32_t shuffle_seed) {
+    if (!G.up) { set_error("qw_kv8_arena_alloc before qw_gpu_init"); return nullptr; }
+    return arena_new(nullptr, true, n_layers, kv_heads, max_ctx, head_dim, shuffle_seed, 1);
+}
+extern "C" qw_buf qw_kv8_arena_alloc_in(qw_buf pool, int32_t n_layers, int32_t kv_heads, int32_t max_ctx, int32_t head_dim) {
+    if (!pool || pool->kind != BUF_POOL) { set_error("qw_kv8_arena_alloc_in: not a pool"); return nullptr; }
+    use_device(pool->device);
+    return arena_new(pool->pool, false, n_layers, kv_heads, max_ctx, head_dim, 0, 1);
+}
 extern "C" int64_t qw_kv_pool_bytes_committed(qw_buf pool) {
     if (!pool || pool->kind != BUF_POOL) return -1;
     return pool->pool->vmm ? (int64_t)(pool->pool->chunks.size() * CHUNK_BYTES) : (int64_t)pool->pool->va_size;
@@ -992,6 +1117,7 @@ static bool kv_rw(qw_buf cache, int32_t layer, int32_t head, int32_t pos0, int32
     const size_t row = (size_t)head_dim * 2;
     if (cache->kind == BUF_ARENA) {
         Arena *a = cache->arena;
+        if (a->elem_bytes != 2) { set_error("qw_kv_read/store: an 8-bit arena is read with qw_op_kv8_read"); return false; }
         if (a->kv_heads != kv_heads || a->max_ctx != max_ctx || layer < 0 || layer >= a->n_layers) { set_error("qw_kv_read/store: shape differs from the arena's"); return false; }
         use_device(cache->device);
         if (store && !arena_ensure(a, layer, pos0, pos0 + n, 0)) return false;
@@ -1089,7 +1215,7 @@ extern "C" void qw_kv_arena_trim(qw_buf cache, int32_t n_tokens) {
     Arena *a = cache->arena;
     use_device(cache->device);
     cudaDeviceSynchronize();
-    const int keep = (std::max(n_tokens, 0) + QW_PAGE_TOKENS - 1) / QW_PAGE_TOKENS;
+    const int keep = (std::max(n_tokens, 0) + a->page_tokens - 1) / a->page_tokens;
     for (size_t lh = 0; lh < (size_t)a->n_layers * a->kv_heads; lh++) {
         int32_t *row = a->table_host.data() + lh * a->pages_per_head;
         bool any = false;
@@ -1850,6 +1976,280 @@ extern "C" bool qw_op_attn_preop(qw_cmd c, qw_ref q_out, qw_ref qg, qw_ref k, qw
     if (!qo) return false;
     FusedSeq s = {qw_ref{nullptr, 0}, qg, k, v, pos, kcache, vcache, base_pos};
     return run_preop(c, &s, 1, &qo, q_norm_w, k_norm_w, axis, inv_freq, rows, q_heads, kv_heads, max_ctx, eps, (int)io, append);
+}
+
+// ---------------------------------------------------------------------------------------
+// additive: rotary positions in both layouts, the 8-bit cache and attention over it
+// ---------------------------------------------------------------------------------------
+extern "C" bool qw_rope_scaled_tables(float *inv_freq, float *amp, int32_t rotary_dim, float theta, qw_rope_scaling kind, float factor,
+                                      int32_t original_ctx, float beta_fast, float beta_slow) {
+    if (!inv_freq || rotary_dim <= 0 || (rotary_dim & 1) || !(theta > 0.0f) || !(theta < INFINITY) || !(factor > 0.0f) || !(factor < INFINITY)) {
+        set_error("qw_rope_scaled_tables: bad arguments");
+        return false;
+    }
+    if (kind < QW_ROPE_PLAIN || kind > QW_ROPE_BANDS || (kind == QW_ROPE_NTK && rotary_dim <= 2) ||
+        (kind == QW_ROPE_BANDS && (original_ctx <= 0 || !(theta > 1.0f) || !(factor >= 1.0f) || !(beta_slow > 0.0f) || !(beta_fast > beta_slow)))) {
+        set_error("qw_rope_scaled_tables: this scaling needs other arguments");
+        return false;
+    }
+    const int32_t half = rotary_dim / 2;
+    double base = theta, lo = 0.0, hi = 0.0;
+    if (kind == QW_ROPE_NTK) base *= pow((double)factor, (double)rotary_dim / (rotary_dim - 2));
+    if (kind == QW_ROPE_BANDS) {
+        // pair j turns original_ctx * theta^(-2j / R) / (2 pi) times over the original context: the j of a given count
+        auto pair_of = [&](double turns) { return rotary_dim * log(original_ctx / (turns * 6.283185307179586)) / (2.0 * log((double)theta)); };
+        lo = std::max(floor(pair_of(beta_fast)), 0.0);
+        hi = std::min(ceil(pair_of(beta_slow)), (double)rotary_dim - 1.0);
+        if (hi <= lo) hi = lo + 0.001;
+    }
+    for (int32_t j = 0; j < half; j++) {
+        const double f = pow(base, -2.0 * j / rotary_dim);
+        double v = f;
+        if (kind == QW_ROPE_LINEAR) v = f / factor;
+        if (kind == QW_ROPE_BANDS) {
+            const double slow = std::min(std::max((j - lo) / (hi - lo), 0.0), 1.0);
+            v = f * (1.0 - slow) + f / factor * slow;
+        }
+        inv_freq[j] = (float)v;
+    }
+    if (amp) *amp = kind == QW_ROPE_BANDS ? (float)(0.1 * log((double)factor) + 1.0) : 1.0f;
+    return true;
+}
+
+extern "C" bool qw_op_rope(qw_cmd c, qw_ref y, qw_ref x, qw_ref pos, qw_ref inv_freq, int32_t rows, int32_t heads, int32_t head_dim,
+                           int32_t rotary_dim, qw_rope_layout layout, int64_t y_stride, int64_t x_stride, float amp, qw_dtype io) {
+    if (!live(c) || rows < 0) return false;
+    if (heads <= 0 || heads > 65535 || head_dim <= 0 || head_dim > 4096 || rotary_dim <= 0 || (rotary_dim & 1) || rotary_dim > head_dim ||
+        (layout != QW_ROPE_HALF && layout != QW_ROPE_INTERLEAVED) || (io != QW_F32 && io != QW_BF16)) {
+        cmd_fail(c, "rope: heads %d, head_dim %d, rotary_dim %d, layout %d, type %d not supported", heads, head_dim, rotary_dim, (int)layout, (int)io);
+        return false;
+    }
+    const int64_t width = (int64_t)heads * head_dim;
+    if (x_stride < width || y_stride < width || x_stride > 0x7fffffff || y_stride > 0x7fffffff) {
+        cmd_fail(c, "rope: row strides %lld and %lld for rows of %lld", (long long)y_stride, (long long)x_stride, (long long)width);
+        return false;
+    }
+    if (rows == 0) return true;
+    const size_t el = io == QW_BF16 ? 2 : 4;
+    const size_t xn = ((size_t)(rows - 1) * x_stride + width) * el, yn = ((size_t)(rows - 1) * y_stride + width) * el;
+    RopeParams p;
+    p.x = near_range(c, x, xn, false);
+    p.y = near_range(c, y, yn, true);
+    p.pos = (const int32_t *)near_range(c, pos, (size_t)rows * 4, false, 4);
+    p.inv_freq = (const float *)near_range(c, inv_freq, (size_t)(rotary_dim / 2) * 4, false, 4);
+    if (!p.x || !p.y || !p.pos || !p.inv_freq) return false;
+    const uintptr_t xa = (uintptr_t)p.x, ya = (uintptr_t)p.y;
+    if (xa < ya + yn && ya < xa + xn && (xa != ya || x_stride != y_stride)) {
+        cmd_fail(c, "rope: the output overlaps the input without being the same rows");
+        return false;
+    }
+    p.y_stride = y_stride; p.x_stride = x_stride;
+    p.rows = rows; p.heads = heads; p.head_dim = head_dim; p.rotary_dim = rotary_dim;
+    p.interleaved = layout == QW_ROPE_INTERLEAVED; p.io = io; p.amp = amp;
+    launch_rope(c->stream, p);
+    return cuda_ok(c, cudaGetLastError(), "rope launch");
+}
+
+namespace {
+
+bool kv8_shape(qw_cmd c, const char *op, int32_t kv_heads, int32_t head_dim, int32_t max_ctx, qw_dtype io) {
+    if (kv_heads > 0 && kv_heads <= 32767 && head_dim == QW_HEAD_DIM && max_ctx > 0 && (int64_t)kv_heads * max_ctx <= 0x7fffffff &&
+        (io == QW_F32 || io == QW_BF16)) return true;
+    cmd_fail(c, "%s: kv_heads %d, head_dim %d, max_ctx %d, type %d not supported", op, kv_heads, head_dim, max_ctx, (int)io);
+    return false;
+}
+bool same_ref(qw_ref a, qw_ref b) { return a.buf == b.buf && a.off == b.off; }
+
+bool kv8_write(qw_cmd c, int n_seq, const qw_ref *kcache, const qw_ref *vcache, const qw_ref *k, const qw_ref *v, const int32_t *base_pos,
+               int32_t rows, int32_t kv_heads, int32_t head_dim, int32_t max_ctx, int64_t row_stride, qw_dtype io) {
+    if (!kv8_shape(c, "kv8_write", kv_heads, head_dim, max_ctx, io)) return false;
+    const int64_t width = (int64_t)kv_heads * QW_HEAD_DIM;
+    const size_t el = io == QW_BF16 ? 2 : 4;
+    if (row_stride < width || row_stride > 0x7fffffff || row_stride * el % 16) {
+        cmd_fail(c, "kv8_write: row stride %lld (rows of %lld elements, a multiple of 16 bytes)", (long long)row_stride, (long long)width);
+        return false;
+    }
+    for (int i = 0; i < n_seq; i++) {
+        if (base_pos[i] < 0 || (int64_t)base_pos[i] + rows > max_ctx) {
+            cmd_fail(c, "kv8_write: positions [%d, %lld) outside the cache", base_pos[i], (long long)base_pos[i] + rows);
+            return false;
+        }
+        for (int j = 0; j <= i; j++)
+            if (same_ref(kcache[i], vcache[j]) || same_ref(vcache[i], kcache[j]) || (j < i && (same_ref(kcache[i], kcache[j]) || same_ref(vcache[i], vcache[j])))) {
+                cmd_fail(c, "kv8_write: one cache appears twice in a call");
+                return false;
+            }
+    }
+    if (rows == 0) return true;
+    const size_t bytes = ((size_t)(rows - 1) * row_stride + width) * el;
+    for (int s0 = 0; s0 < n_seq; s0 += QW_MAX_SEQ) {
+        Kv8WriteParams p;
+        memset(&p, 0, sizeof p);
+        p.n_seq = std::min(QW_MAX_SEQ, n_seq - s0);
+        for (int i = 0; i < p.n_seq; i++) {
+            Kv8WriteSeq &q = p.seq[i];
+            const int32_t b = base_pos[s0 + i];
+            q.base_pos = b;
+            q.k = near_range(c, k[s0 + i], bytes, false);
+            q.v = near_range(c, v[s0 + i], bytes, false);
+            if (!q.k || !q.v) return false;
+            if (!resolve_kv8(c, kcache[s0 + i], kv_heads, max_ctx, b, b + rows, true, &q.kc, nullptr) ||
+                !resolve_kv8(c, vcache[s0 + i], kv_heads, max_ctx, b, b + rows, true, &q.vc, nullptr)) return false;
+            p.max_blocks = std::max(p.max_blocks, (b + rows - 1) / QW_KV8_BLOCK - b / QW_KV8_BLOCK + 1);
+        }
+        p.row_stride = row_stride; p.rows = rows; p.kv_heads = kv_heads; p.io = io;
+        p.status = cmd_status(c);
+        launch_kv8_write(c->stream, p);
+        if (!cuda_ok(c, cudaGetLastError(), "kv8_write launch")) return false;
+    }
+    return true;
+}
+
+struct Kv8Call {
+    qw_ref out, gate, q, kcache, vcache;
+    int32_t base_pos;
+};
+
+// Many bf16 rows: the cache is widened to bf16 once (a code times a power of two is a bf16 number) and the tcgen05
+// prefill kernel runs over the copy.
+bool kv8_prefill(qw_cmd c, const Kv8Layer &kc, const Kv8Layer &vc, const void *q, void *out, const void *gate, int32_t rows, int32_t q_heads,
+                 int32_t kv_heads, int32_t base_pos, float scale, int32_t gate_stride) {
+    const int n = base_pos + rows;
+    const size_t one = (size_t)kv_heads * n * QW_HEAD_DIM * 2;
+    char *scr = (char *)cmd_scratch(c, 2 * one);
+    if (!scr) return false;
+    launch_kv8_read(c->stream, scr, DT_BF16, kc, kv_heads, 0, n);
+    launch_kv8_read(c->stream, scr + one, DT_BF16, vc, kv_heads, 0, n);
+    PrefillParams p;
+    memset(&p, 0, sizeof p);
+    const int64_t map_rows = (int64_t)kv_heads * n;
+    if (!encode_rows_map(&p.kmap, scr, map_rows, 64) || !encode_rows_map(&p.vmap, scr + one, map_rows, 64))
+        return cmd_fail(c, "%s", SH.last_error), false;
+    p.kc.base = reinterpret_cast<__nv_bfloat16 *>(scr); p.kc.max_ctx = n;
+    p.vc.base = reinterpret_cast<__nv_bfloat16 *>(scr + one); p.vc.max_ctx = n;
+    return run_prefill_on(c, p, map_rows, map_rows, reinterpret_cast<const __nv_bfloat16 *>(q), out, DT_BF16, gate, DT_BF16, gate_stride, rows,
+                          q_heads, kv_heads, base_pos, scale);
+}
+
+bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_ctx,
+              float scale, int32_t gate_stride, qw_dtype io) {
+    if (!kv8_shape(c, "attn_kv8", kv_heads, head_dim, max_ctx, io)) return false;
+    const int most = kv8_max_query_rows(io), gqa = q_heads > 0 ? q_heads / kv_heads : 0;
+    if (q_heads <= 0 || q_heads % kv_heads || gqa > most) { cmd_fail(c, "attn_kv8: %d query heads over %d (at most %d to one) not supported", q_heads, kv_heads, most); return false; }
+    const size_t el = io == QW_BF16 ? 2 : 4;
+    for (int i = 0; i < n_seq; i++) {
+        if (calls[i].base_pos < 0 || (int64_t)calls[i].base_pos + rows > max_ctx) {
+            cmd_fail(c, "attn_kv8: positions [%d, %lld) outside the cache", calls[i].base_pos, (long long)calls[i].base_pos + rows);
+            return false;
+        }
+        if (calls[i].gate.buf && gate_stride < QW_HEAD_DIM) { cmd_fail(c, "attn_kv8: gate stride %d", gate_stride); return false; }
+        for (int j = 0; j < i; j++)
+            if (rows > 0 && same_ref(calls[i].out, calls[j].out)) { cmd_fail(c, "attn_kv8: one output appears twice in a call"); return false; }
+    }
+    if (rows == 0) return true;
+    const size_t n = (size_t)rows * q_heads, bytes = n * QW_HEAD_DIM * el;
+    const int chunk = std::max(1, most / gqa);
+    Kv8AttnParams p;
+    memset(&p, 0, sizeof p);
+    p.q_heads = q_heads; p.kv_heads = kv_heads; p.gqa = gqa; p.io = io; p.gate_stride = gate_stride; p.scale = scale;
+    int n_maps = 0, max_rows = 0;
+    int64_t tiles = 0;
+    auto flush = [&]() {
+        if (!p.n_seq) return true;
+        kv8_attn_plan(p);
+        void *scr = cmd_scratch(c, kv8_attn_scratch_bytes(p));
+        if (!scr) return false;
+        p.status = cmd_status(c);
+        launch_kv8_attn(c->stream, p, max_rows, scr);
+        p.n_seq = 0; n_maps = 0; max_rows = 0; tiles = 0;
+        return cuda_ok(c, cudaGetLastError(), "attn_kv8 launch");
+    };
+    auto map_slot = [&](const CUtensorMap &m) {
+        for (int i = 0; i < n_maps; i++)
+            if (!memcmp(&p.maps[i], &m, sizeof m)) return i;
+        if (n_maps == QW_MAX_MAPS) return -1;
+        p.maps[n_maps] = m;
+        return n_maps++;
+    };
+    for (int i = 0; i < n_seq; i++) {
+        const Kv8Call &a = calls[i];
+        Kv8Layer kc, vc;
+        CUtensorMap km, vm;
+        const int32_t end = a.base_pos + rows;
+        if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &kc, &km) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &vc, &vm)) return false;
+        const char *qp = (const char *)near_range(c, a.q, bytes, false);
+        char *op = (char *)near_range(c, a.out, bytes, true);
+        const char *gp = a.gate.buf ? (const char *)near_range(c, a.gate, ((n - 1) * gate_stride + QW_HEAD_DIM) * el, false) : nullptr;
+        if (!qp || !op || (a.gate.buf && !gp)) return false;
+        if (rows * gqa > most && io == QW_BF16 && attn_prefill_io_ok(op, DT_BF16, gp, DT_BF16, gate_stride)) {
+            if (!flush()) return false;
+            if (!kv8_prefill(c, kc, vc, qp, op, gp, rows, q_heads, kv_heads, a.base_pos, scale, gate_stride)) return false;
+            continue;
+        }
+        for (int r0 = 0; r0 < rows; r0 += chunk) {
+            const int rr = std::min(chunk, rows - r0);
+            const int64_t add = (int64_t)((a.base_pos + r0 + rr + 31) / 32) * kv_heads;
+            int ks = -1, vs = -1;
+            for (int attempt = 0; attempt < 2 && vs < 0; attempt++) {
+                if (attempt && !flush()) return false;
+                if (p.n_seq == QW_MAX_SEQ || tiles + add > 0x3fffffff) continue;
+                const int saved = n_maps;
+                ks = map_slot(km);
+                vs = ks < 0 ? -1 : map_slot(vm);
+                if (vs < 0) n_maps = saved;
+            }
+            if (vs < 0) { cmd_fail(c, "attn_kv8: the call does not fit a launch"); return false; }
+            Kv8AttnSeq &s = p.seq[p.n_seq++];
+            memset(&s, 0, sizeof s);
+            s.q = qp + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
+            s.out = op + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
+            s.gate = gp ? gp + (size_t)r0 * q_heads * gate_stride * el : nullptr;
+            s.kc = kc; s.vc = vc; s.rows = rr; s.base_pos = a.base_pos + r0;
+            s.kmap = (uint8_t)ks; s.vmap = (uint8_t)vs;
+            max_rows = std::max(max_rows, rr);
+            tiles += add;
+        }
+    }
+    return flush();
+}
+
+}  // namespace
+
+extern "C" bool qw_op_kv8_write(qw_cmd c, qw_ref kcache, qw_ref vcache, qw_ref k, qw_ref v, int32_t rows, int32_t kv_heads, int32_t head_dim,
+                                int32_t max_ctx, int32_t base_pos, int64_t row_stride, qw_dtype io) {
+    if (!live(c) || rows < 0) return false;
+    return kv8_write(c, 1, &kcache, &vcache, &k, &v, &base_pos, rows, kv_heads, head_dim, max_ctx, row_stride, io);
+}
+extern "C" bool qw_op_kv8_write_batch(qw_cmd c, int32_t n_seq, const qw_ref *kcache, const qw_ref *vcache, const qw_ref *k, const qw_ref *v,
+                                      const int32_t *base_pos, int32_t rows, int32_t kv_heads, int32_t head_dim, int32_t max_ctx,
+                                      int64_t row_stride, qw_dtype io) {
+    if (!live(c) || rows < 0 || n_seq < 0 || (n_seq && (!kcache || !vcache || !k || !v || !base_pos))) return false;
+    return kv8_write(c, n_seq, kcache, vcache, k, v, base_pos, rows, kv_heads, head_dim, max_ctx, row_stride, io);
+}
+extern "C" bool qw_op_kv8_read(qw_cmd c, qw_ref dst, qw_ref cache, int32_t pos0, int32_t n, int32_t kv_heads, int32_t head_dim, int32_t max_ctx,
+                               qw_dtype io) {
+    if (!live(c) || n < 0 || !kv8_shape(c, "kv8_read", kv_heads, head_dim, max_ctx, io)) return false;
+    if (pos0 < 0 || (int64_t)pos0 + n > max_ctx) { cmd_fail(c, "kv8_read: positions [%d, %lld) outside the cache", pos0, (long long)pos0 + n); return false; }
+    if (n == 0) return true;
+    Kv8Layer L;
+    void *d = near_range(c, dst, (size_t)kv_heads * n * QW_HEAD_DIM * (io == QW_BF16 ? 2 : 4), true);
+    if (!d || !resolve_kv8(c, cache, kv_heads, max_ctx, pos0, pos0 + n, false, &L, nullptr)) return false;
+    launch_kv8_read(c->stream, d, io, L, kv_heads, pos0, n);
+    return cuda_ok(c, cudaGetLastError(), "kv8_read launch");
+}
+extern "C" bool qw_op_attn_kv8(qw_cmd c, qw_ref out, qw_ref gate, qw_ref q, qw_ref kcache, qw_ref vcache, int32_t rows, int32_t q_heads,
+                               int32_t kv_heads, int32_t head_dim, int32_t max_ctx, int32_t base_pos, float scale, int32_t gate_stride, qw_dtype io) {
+    if (!live(c) || rows < 0) return false;
+    const Kv8Call a = {out, gate, q, kcache, vcache, base_pos};
+    return attn_kv8(c, &a, 1, rows, q_heads, kv_heads, head_dim, max_ctx, scale, gate_stride, io);
+}
+extern "C" bool qw_op_attn_kv8_batch(qw_cmd c, int32_t n_seq, const qw_ref *out, const qw_ref *gate, const qw_ref *q, const qw_ref *kcache,
+                                     const qw_ref *vcache, const int32_t *base_pos, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                                     int32_t head_dim, int32_t max_ctx, float scale, int32_t gate_stride, qw_dtype io) {
+    if (!live(c) || rows < 0 || n_seq < 0 || (n_seq && (!out || !q || !kcache || !vcache || !base_pos))) return false;
+    std::vector<Kv8Call> calls((size_t)n_seq);
+    for (int32_t i = 0; i < n_seq; i++) calls[(size_t)i] = Kv8Call{out[i], gate ? gate[i] : qw_ref{nullptr, 0}, q[i], kcache[i], vcache[i], base_pos[i]};
+    return attn_kv8(c, calls.data(), n_seq, rows, q_heads, kv_heads, head_dim, max_ctx, scale, gate_stride, io);
 }
 
 extern "C" bool qw_op_attn_partial(qw_cmd c, qw_ref pacc, qw_ref pstat, qw_ref q, qw_ref kcache, qw_ref vcache, int32_t rows,
