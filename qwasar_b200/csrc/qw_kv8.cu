@@ -633,6 +633,339 @@ __global__ void __launch_bounds__(AT_THREADS, 1) kv8_attn_kernel(const __grid_co
         for (int i = 0; i < 4096; i++) __nanosleep(10000);
 }
 
+// =======================================================================================
+// attention, up to eight query rows (a decode step)
+// =======================================================================================
+// The same line of tiles, shares and rings, with the products turned over: S^T = K Q^T and O^T = V^T P^T, so that the
+// cache is the 16-row operand of the tensor op and the query rows its eight columns.  With Q as the 16-row operand
+// half of every tensor op would multiply padding, and the running output would take 128 registers a thread instead of
+// 64; at 64, twelve warps fit an SM instead of eight, and the kernel stops waiting on its own instruction latency.
+// f32 rows put their high and low parts through the same accumulators one after the other.
+// The weights come out with a key per lane group and are wanted with a query row there: movmatrix turns an 8 x 8 block.
+constexpr int D_WARPS = 12, D_THREADS = D_WARPS * 32, D_NS = 2;
+constexpr int D_OFF_Q = D_WARPS * D_NS * ENTRY;
+constexpr int D_OFF_M = D_OFF_Q + 8192;                   // [warp][8]
+constexpr int D_OFF_L = D_OFF_M + D_WARPS * 32;
+constexpr int D_OFF_QE = D_OFF_L + D_WARPS * 32;          // [8]
+constexpr int D_OFF_BAR = D_OFF_QE + 32;                  // full[warps * slots], abort
+constexpr int D_SMEM = D_OFF_BAR + D_WARPS * D_NS * 8 + 16;
+static_assert(D_SMEM <= 232448, "exceeds the 227 KB a CTA may use");
+
+__device__ __forceinline__ uint32_t movm(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_constant__ Kv8AttnParams p) {
+    constexpr int KG = D_WARPS, NS = D_NS;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    float *sm_m = reinterpret_cast<float *>(smem + D_OFF_M);
+    float *sm_l = reinterpret_cast<float *>(smem + D_OFF_L);
+    int *sm_qe = reinterpret_cast<int *>(smem + D_OFF_QE);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + D_OFF_BAR);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(full + KG * NS);
+
+    if (smem_u32(smem) & 1023u) {                    // swizzled boxes need 1024-byte alignment
+        if (threadIdx.x == 0) report(p.status, QW_ST_BAD_SMEM);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < KG * NS; i++) mbar_init(&full[i], 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_next();
+
+    uint8_t *ring = smem + warp * NS * ENTRY;
+    full += warp * NS;
+    const int lo = share_lo(p, blockIdx.x), hi = share_lo(p, blockIdx.x + 1);
+    Where w = locate(p, lo);
+    uint32_t phase = 0;                              // of both slots: K in slot 0, V in slot 1
+
+    for (int T = lo; T < hi;) {
+        const Kv8AttnSeq &sq = p.seq[w.s];
+        const int seg_t0 = w.t, seg_n = min(sq.n_tiles - w.t, hi - T);
+        const int valid = sq.rows * p.gqa, head0 = w.h * p.gqa;
+        const int n_keys = sq.base_pos + sq.rows;
+        const int nt = warp < seg_n ? (seg_n - warp + KG - 1) / KG : 0;      // this warp's tiles
+
+        int win_k = 0, win_v = 0, win_e = 0;         // code rows and exponents of 32 tiles, one per lane
+        auto window = [&](int i0) {
+            const int i = i0 + lane;
+            if (i < nt) {
+                const int key = (seg_t0 + warp + i * KG) * TILE;
+                const int64_t kr = code_row(sq.kc, w.h, key), vr = code_row(sq.vc, w.h, key);
+                if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
+                win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
+                const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key / BLK]);
+                const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key / BLK]);
+                win_e = (ek & 0xffff) | (ev << 16);
+            }
+        };
+        auto load = [&](int row, int is_v) {         // lane 0
+            mbar_expect_tx(&full[is_v], ENTRY);
+            const CUtensorMap *map = &p.maps[is_v ? sq.vmap : sq.kmap];
+            tma_load_2d(ring + is_v * ENTRY, map, 0, row, &full[is_v]);
+            tma_load_2d(ring + is_v * ENTRY + BOX, map, 128, row, &full[is_v]);
+        };
+        if (nt > 0) {
+            window(0);
+            if (lane == 0) { load(win_k, 0); load(win_v, 1); }
+        }
+
+        // ---- Q: one warp per row, 8 dims per lane, scaled below 2^14 and put where the B fragments are read: step
+        // 4 q + i takes dims 64 q + 16 t + 4 i + {0, 1 | 2, 3} of row g in lane (g, t) ----
+        for (int row = warp; row < 8; row += D_WARPS) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = 0.0f;
+            if (row < valid) {
+                const int r = row / p.gqa, hh = row - r * p.gqa;
+                const size_t at = ((size_t)r * p.q_heads + head0 + hh) * 256 + lane * 8;
+                if constexpr (F32) {
+                    const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at);
+                    const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at + 4);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                } else {
+                    const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(sq.q) + at);
+                    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
+                }
+            }
+            float mx = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
+            mx = warp_max(mx);
+            const int qe = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 13, -100), 100);
+            const float f = pow2f(-qe);
+            if (lane == 0) sm_qe[row] = qe;
+            uint32_t hp[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) { x[2 * k] *= f; x[2 * k + 1] *= f; hp[k] = pack_f16(x[2 * k], x[2 * k + 1]); }
+            const int q = lane >> 3, tt = (lane >> 1) & 3;
+            if constexpr (F32) {
+                uint32_t lp[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) { const float2 h = h2f2(hp[k]); lp[k] = pack_f16(x[2 * k] - h.x, x[2 * k + 1] - h.y); }
+                uint4 *fr = reinterpret_cast<uint4 *>(smem + D_OFF_Q) + (q * 4 + (lane & 1) * 2) * 32 + row * 4 + tt;
+                fr[0] = make_uint4(hp[0], hp[1], lp[0], lp[1]);
+                fr[32] = make_uint4(hp[2], hp[3], lp[2], lp[3]);
+            } else {
+                reinterpret_cast<uint4 *>(smem + D_OFF_Q)[(q * 2 + (lane & 1)) * 32 + row * 4 + tt] = make_uint4(hp[0], hp[1], hp[2], hp[3]);
+            }
+        }
+        __syncthreads();
+
+        float o[16][4];
+#pragma unroll
+        for (int n = 0; n < 16; n++) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
+        // this thread's columns: query rows 2 t and 2 t + 1
+        const int row0 = 2 * t, row1 = row0 + 1;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        const int lim0 = row0 < valid ? sq.base_pos + row0 / p.gqa : n_keys - 1;
+        const int lim1 = row1 < valid ? sq.base_pos + row1 / p.gqa : n_keys - 1;
+        const float sc0 = p.scale * LOG2E * pow2f(sm_qe[row0]), sc1 = p.scale * LOG2E * pow2f(sm_qe[row1]);
+        const uint32_t q_base = smem_u32(smem + D_OFF_Q) + lane * 16;
+        const uint32_t tok = (uint32_t)(g ^ ((g & 1) << 2));         // this lane group's key of a block of eight
+        const uint32_t k_base = smem_u32(ring) + tok * 128, v_base = smem_u32(ring + ENTRY);
+
+#pragma unroll 1
+        for (int i = 0; i < nt; i++, phase ^= 1) {
+            const int key0 = (seg_t0 + warp + i * KG) * TILE;
+            const int ex = __shfl_sync(0xffffffffu, win_e, i & 31);
+            const int ek = (int)(int16_t)(ex & 0xffff), ev = ex >> 16;
+            if (i + 1 < nt && ((i + 1) & 31) == 0) window(i + 1);
+            const int nk = __shfl_sync(0xffffffffu, win_k, (i + 1) & 31), nv = __shfl_sync(0xffffffffu, win_v, (i + 1) & 31);
+
+            // ---- S^T = K Q^T ----
+            float s[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            mbar_wait(&full[0], phase, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                uint32_t kw[4][4];                     // keys tok, tok + 8, tok + 16, tok + 24
+#pragma unroll
+                for (int n = 0; n < 4; n++) lds128(kw[n], k_base + (q >> 1) * BOX + n * 1024 + ((((uint32_t)(4 * (q & 1) + t)) ^ tok) << 4));
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+                    uint32_t qf[2][4];
+                    if constexpr (F32) { lds128(qf[0], q_base + (q * 4 + kk * 2) * 512); lds128(qf[1], q_base + (q * 4 + kk * 2 + 1) * 512); }
+                    else lds128(qf[0], q_base + (q * 2 + kk) * 512);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int k = kk * 2 + h;
+#pragma unroll
+                        for (int n = 0; n < 2; n++) {
+                            const uint32_t a0 = f16x2_lo(kw[2 * n][k]), a1 = f16x2_lo(kw[2 * n + 1][k]), a2 = f16x2_hi(kw[2 * n][k]), a3 = f16x2_hi(kw[2 * n + 1][k]);
+                            if constexpr (F32) {
+                                mma_f16(s[n], a0, a1, a2, a3, qf[h][0], qf[h][1]);
+                                mma_f16(s[n], a0, a1, a2, a3, qf[h][2], qf[h][3]);
+                            } else {
+                                mma_f16(s[n], a0, a1, a2, a3, qf[0][2 * h], qf[0][2 * h + 1]);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0 && i + 1 < nt) load(nk, 0);
+
+            // ---- online softmax ----
+            const float k0 = sc0 * pow2f(ek), k1 = sc1 * pow2f(ek), fv = (float)ev;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[n][c] = fmaf(s[n][c], (c & 1) ? k1 : k0, fv);
+            if (key0 + TILE > sq.base_pos + 1) {
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (key0 + n * 16 + (c >> 1) * 8 + (int)tok > ((c & 1) ? lim1 : lim0)) s[n][c] = -INFINITY;
+            }
+            float x0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
+            float x1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+            }
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                const float f0 = m0 == n0 ? 1.0f : ex2(m0 - n0), f1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
+                l0 *= f0; l1 *= f1;
+#pragma unroll
+                for (int n = 0; n < 16; n++) { o[n][0] *= f0; o[n][1] *= f1; o[n][2] *= f0; o[n][3] *= f1; }
+                m0 = n0; m1 = n1;
+            }
+            const float b0 = (m0 == -INFINITY ? 0.0f : m0) - W_SHIFT, b1 = (m1 == -INFINITY ? 0.0f : m1) - W_SHIFT;
+            uint32_t pb[2][2], pl[2][2];               // B fragments of the weights (f32: high and low parts)
+            float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float w0 = ex2(s[n][2 * c] - b0), w1 = ex2(s[n][2 * c + 1] - b1);
+                    a0 += w0; a1 += w1;
+                    const uint32_t hi = pack_f16(w0, w1);
+                    pb[n][c] = movm(hi);
+                    if constexpr (F32) {
+                        const float2 h = h2f2(hi);
+                        pl[n][c] = movm(pack_f16(w0 - h.x, w1 - h.y));
+                    }
+                }
+            const float iv = pow2f(-ev);
+            l0 = fmaf(a0, iv, l0); l1 = fmaf(a1, iv, l1);
+
+            // ---- O^T += V^T P^T: row g of tile 8 x + j is dim 128 x + 16 g + 2 j, row g + 8 the dim after it; the two
+            // keys of a register are interleaved byte by byte before they are widened ----
+            mbar_wait(&full[1], phase, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            if (key0 + TILE > n_keys) {                // rows past the last key may hold anything
+                for (int off = (n_keys - key0) * 128 + lane * 16; off < TILE * 128; off += 512) {
+                    *reinterpret_cast<uint4 *>(ring + ENTRY + off) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(ring + ENTRY + BOX + off) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+                __syncwarp();
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const uint32_t ta = 16 * n + 2 * t, tb = 16 * n + ((2 * t + 1) ^ 4);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    uint32_t v[4][4];                  // keys ta, tb, ta + 8, tb + 8
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t tk = ((c & 1) ? tb : ta) + (c >> 1) * 8;
+                        lds128(v[c], v_base + x * BOX + tk * 128 + (((uint32_t)g ^ (tk & 7)) << 4));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140), p1 = __byte_perm(v[0][k], v[1][k], 0x7362);
+                        const uint32_t r0 = __byte_perm(v[2][k], v[3][k], 0x5140), r1 = __byte_perm(v[2][k], v[3][k], 0x7362);
+                        const uint32_t c0 = f16x2_lo(p0), c1 = f16x2_hi(p0), c2 = f16x2_lo(r0), c3 = f16x2_hi(r0);
+                        const uint32_t d0 = f16x2_lo(p1), d1 = f16x2_hi(p1), d2 = f16x2_lo(r1), d3 = f16x2_hi(r1);
+                        mma_f16(o[x * 8 + 2 * k], c0, c1, c2, c3, pb[n][0], pb[n][1]);
+                        mma_f16(o[x * 8 + 2 * k + 1], d0, d1, d2, d3, pb[n][0], pb[n][1]);
+                        if constexpr (F32) {
+                            mma_f16(o[x * 8 + 2 * k], c0, c1, c2, c3, pl[n][0], pl[n][1]);
+                            mma_f16(o[x * 8 + 2 * k + 1], d0, d1, d2, d3, pl[n][0], pl[n][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0 && i + 1 < nt) load(nv, 1);
+        }
+
+        // ---- segment end: every warp puts its sums into its first slot, and all threads add them up ----
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+        }
+        if (g == 0) { sm_m[warp * 8 + row0] = m0; sm_m[warp * 8 + row1] = m1; sm_l[warp * 8 + row0] = l0; sm_l[warp * 8 + row1] = l1; }
+        if (nt > 0) {
+            // piece c (four dims) of a row sits at c ^ ((row >> 1) & 3), which spreads a phase's eight lanes over the banks
+            float *own = reinterpret_cast<float *>(ring);
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int n = x * 8 + 2 * e;
+                    const uint32_t piece = (uint32_t)(x * 32 + g * 4 + e) ^ (uint32_t)t;
+                    *reinterpret_cast<float4 *>(own + row0 * 256 + piece * 4) = make_float4(o[n][0], o[n][2], o[n + 1][0], o[n + 1][2]);
+                    *reinterpret_cast<float4 *>(own + row1 * 256 + piece * 4) = make_float4(o[n][1], o[n][3], o[n + 1][1], o[n + 1][3]);
+                }
+        }
+        __syncthreads();
+        const bool whole = seg_t0 == 0 && seg_n == sq.n_tiles;
+        const size_t slot = (size_t)blockIdx.x + (size_t)w.s * p.kv_heads + w.h;
+        const int in = min(KG, seg_n);                 // warps that had a tile
+        for (int idx = threadIdx.x; idx < valid * 64; idx += D_THREADS) {
+            const int row = idx >> 6, pc = idx & 63;
+            const uint32_t piece = (uint32_t)pc ^ (uint32_t)((row >> 1) & 3);
+            float M = -INFINITY;
+            for (int k = 0; k < in; k++) M = fmaxf(M, sm_m[k * 8 + row]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.0f;
+            for (int k = 0; k < in; k++) {
+                const float mk = sm_m[k * 8 + row], f = mk == M ? 1.0f : ex2(mk - M);
+                const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + k * NS * ENTRY) + row * 256 + piece * 4);
+                L = fmaf(sm_l[k * 8 + row], f, L);
+                acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y); acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+            }
+            if (whole) {
+                const int r = row / p.gqa;
+                const float inv = 1.0f / L;
+                store_out(p, sq, (size_t)r * p.q_heads + head0 + (row - r * p.gqa), pc * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+            } else {
+                const size_t pi = slot * p.slot_rows + row;
+                *reinterpret_cast<float4 *>(p.pacc + pi * 256 + pc * 4) = acc;
+                if (pc == 0) *reinterpret_cast<float2 *>(p.pstat + pi * 2) = make_float2(M, L);
+            }
+        }
+        T += seg_n;
+        w.t = 0;                                          // the next segment, if any, begins the next group
+        if (++w.h == p.kv_heads) { w.h = 0; w.s++; }
+        fence_proxy_async();                              // the ring goes back to the copy engine
+        __syncthreads();
+    }
+    if (*abort_flag)                                      // a wait gave up: copies of this CTA may still be under way
+        for (int i = 0; i < 4096; i++) __nanosleep(10000);
+}
+
 // Partials of a cut group: one block per (group, row); the four quarters of the block take every fourth partial.
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const __grid_constant__ Kv8AttnParams p, int max_valid) {
     __shared__ float w_s[256];
@@ -712,6 +1045,22 @@ void launch_attn_t(cudaStream_t s, const Kv8AttnParams &p) {
     g_launches++;
 }
 
+template <bool F32>
+void launch_decode_t(cudaStream_t s, const Kv8AttnParams &p) {
+    static bool configured[64] = {false};      // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !configured[dev]) {
+        cudaFuncSetAttribute(kv8_decode_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, D_SMEM);
+        configured[dev] = true;
+    }
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(cfg, attr, dim3((unsigned)p.n_cta), D_THREADS, D_SMEM, s);
+    cudaLaunchKernelEx(&cfg, kv8_decode_kernel<F32>, p);
+    g_launches++;
+}
+
 }  // namespace
 
 void launch_kv8_write(cudaStream_t s, const Kv8WriteParams &p) {
@@ -757,6 +1106,8 @@ void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scrat
     p.pstat = p.pacc + slots * p.slot_rows * 256;
     const int valid = max_rows * p.gqa, f32 = p.io == DT_F32, per = f32 ? 8 : 16;
     const int mt = (valid + per - 1) / per;
+    if (valid <= 8) { if (f32) launch_decode_t<true>(s, p); else launch_decode_t<false>(s, p); }
+    else
     if (f32) { if (mt <= 1) launch_attn_t<1, true>(s, p); else if (mt <= 2) launch_attn_t<2, true>(s, p); else launch_attn_t<4, true>(s, p); }
     else { if (mt <= 1) launch_attn_t<1, false>(s, p); else if (mt <= 2) launch_attn_t<2, false>(s, p); else launch_attn_t<4, false>(s, p); }
     bool cut = false;
