@@ -269,6 +269,7 @@ struct Kv8AttnParams {
     Kv8AttnSeq seq[QW_MAX_SEQ];
     int32_t n_seq, q_heads, kv_heads, gqa;
     int32_t total_tiles, n_cta, slot_rows;
+    int32_t share[257];      // CTA c takes tiles [share[c], share[c + 1]) of the line
     int32_t io, gate_stride;
     float scale;
     float *pacc, *pstat;     // partials: [slot, slot_rows, 256] and [slot, slot_rows, 2]; slot = cta + group

@@ -68,11 +68,23 @@ __device__ __forceinline__ int64_t code_row(const Kv8Layer &L, int h, int t) {
 // One CTA per (64-token block, head, K or V, sequence): the block's new rows are read once into registers, their
 // largest magnitude gives the exponent, and the codes leave as whole 256-byte rows.  A block that holds rows already
 // keeps its exponent unless the new rows need a larger one; then its old codes are moved there first.
-constexpr int WR_THREADS = 256;
+constexpr int WR_THREADS = 512, WR_WARPS = WR_THREADS / 32, WR_ROWS = BLK / WR_WARPS;
+
+// Largest of `v` over the block; the same for every thread.
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    __syncthreads();                                         // (of the last use of `red`)
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < WR_WARPS; i++) v = max(v, red[i]);
+    return v;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(WR_THREADS) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
-    __shared__ float red[WR_THREADS / 32];
+    __shared__ uint32_t red[WR_WARPS];
     pdl_wait();
     pdl_launch_next();
     const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
@@ -82,48 +94,52 @@ __global__ void __launch_bounds__(WR_THREADS) kv8_write_kernel(const __grid_cons
     if (first >= last) return;
     const Kv8Layer &L = which ? sq.vc : sq.kc;
     const T *src = reinterpret_cast<const T *>(which ? sq.v : sq.k) + (size_t)h * 256;
+    const int col = (threadIdx.x & 31) * 8, r0 = first + (threadIdx.x >> 5);
+
+    // all of the thread's rows are asked for before the first is looked at: one trip to memory
+    constexpr int RW = sizeof(T) == 2 ? 4 : 8;               // words of eight elements
+    uint32_t raw[WR_ROWS][RW];
+#pragma unroll
+    for (int i = 0; i < WR_ROWS; i++) {
+        const int t = r0 + WR_WARPS * i;
+        const uint4 *g = reinterpret_cast<const uint4 *>(src + (size_t)(t - sq.base_pos) * p.row_stride + col);
+        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        if (t < last) { a = g[0]; if (RW == 8) b = g[1]; }
+        raw[i][0] = a.x; raw[i][1] = a.y; raw[i][2] = a.z; raw[i][3] = a.w;
+        if constexpr (RW == 8) { raw[i][4] = b.x; raw[i][5] = b.y; raw[i][6] = b.z; raw[i][7] = b.w; }
+    }
     const int64_t row0 = code_row(L, h, t0);                 // a block never crosses a page
+    uint8_t *ep = L.exps + (size_t)h * L.exp_stride + blk;
+    const int was = first > t0 ? clamp_exp(*ep) : QW_KV8_E_MIN;
     if (row0 < 0) { if (threadIdx.x == 0) report(p.status, QW_ST_BAD_PAGE); return; }
     uint8_t *dst = L.base + row0 * 256;
-    uint8_t *ep = L.exps + (size_t)h * L.exp_stride + blk;
-    const int col = (threadIdx.x & 31) * 8, r0 = threadIdx.x >> 5;
-
-    float v[8][8];
-    float amax = 0.0f;
-    bool odd = false;                                        // a NaN or an infinity was seen
+    auto element = [&](int i, int e) {
+        if constexpr (RW == 8) return __uint_as_float(raw[i][e]);
+        else return __uint_as_float((e & 1) ? raw[i][e >> 1] & 0xffff0000u : raw[i][e >> 1] << 16);
+    };
+    // magnitudes order like their bits: the largest as a whole number, in the upper half for bf16
+    uint32_t big = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int t = first + r0 + 8 * i;
-        if (t < last) {
-            const T *g = src + (size_t)(t - sq.base_pos) * p.row_stride + col;
-            if constexpr (sizeof(T) == 2) {
-                const uint4 q = *reinterpret_cast<const uint4 *>(g);
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    for (int i = 0; i < WR_ROWS; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) { v[i][2 * e] = __uint_as_float(w[e] << 16); v[i][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
-            } else {
-                const float4 a = *reinterpret_cast<const float4 *>(g), b = *reinterpret_cast<const float4 *>(g + 4);
-                v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
-                v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+        for (int k = 0; k < RW; k++) big = RW == 8 ? max(big, raw[i][k] & 0x7fffffffu) : __vmaxu2(big, raw[i][k] & 0x7fff7fffu);
+    if constexpr (RW == 4) big = max(big & 0xffff0000u, big << 16);
+    // (block_max lies between reading the stored exponent and replacing it)
+    big = block_max(big, red);
+    const bool odd = big >= 0x7f800000u;                     // a NaN or an infinity among them: the largest of the others
+    if (odd) {
+        if (threadIdx.x == 0) report(p.status, QW_ST_KV8_NONFINITE);
+        big = 0;
+#pragma unroll
+        for (int i = 0; i < WR_ROWS; i++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const uint32_t u = __float_as_uint(element(i, k)) & 0x7fffffffu;
+                big = max(big, u < 0x7f800000u ? u : 0u);
             }
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float a = fabsf(v[i][e]);
-                if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
-                else { odd = true; if (a != a) v[i][e] = 0.0f; }       // NaN: stored as zero; infinite: the largest code
-            }
-        }
+        big = block_max(big, red);
     }
-    if (odd) report(p.status, QW_ST_KV8_NONFINITE);
-    amax = warp_max(amax);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-    // (every thread reads the stored exponent before the barrier behind which one of them may replace it)
-    const int was = first > t0 ? clamp_exp(*ep) : QW_KV8_E_MIN;
-    __syncthreads();
-    amax = red[0];
-#pragma unroll
-    for (int i = 1; i < WR_THREADS / 32; i++) amax = fmaxf(amax, red[i]);
-    const int e = max(was, needed_exp(amax));
+    const int e = max(was, needed_exp(__uint_as_float(big)));
     if (first > t0 && e > was) {
         // rows [t0, first): 16 codes to a thread
         const float f = pow2f(max(was - e, -126));
@@ -141,13 +157,17 @@ __global__ void __launch_bounds__(WR_THREADS) kv8_write_kernel(const __grid_cons
     }
     const float inv = pow2f(-e);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int t = first + r0 + 8 * i;
-        if (t < last) {
+    for (int i = 0; i < WR_ROWS; i++) {
+        const int t = r0 + WR_WARPS * i;
+        if (t >= last) break;
+        float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[i][k] *= inv;
-            *reinterpret_cast<uint2 *>(dst + (size_t)(t - t0) * 256 + col) = make_uint2(e4m3x4(v[i]), e4m3x4(v[i] + 4));
+        for (int k = 0; k < 8; k++) v[k] = element(i, k) * inv;
+        if (odd) {                                           // NaN: stored as zero; infinite: the largest code
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = v[k] == v[k] ? v[k] : 0.0f;
         }
+        *reinterpret_cast<uint2 *>(dst + (size_t)(t - t0) * 256 + col) = make_uint2(e4m3x4(v), e4m3x4(v + 4));
     }
     if (threadIdx.x == 0) *ep = (uint8_t)(e + 127);
 }
@@ -239,14 +259,21 @@ struct AtCfg {
     static_assert(AT_WARPS * 16384 <= RING * ENTRY, "the warps' sums do not fit the ring");
 };
 
+#ifndef QW_KV8_SEG_COST
+#define QW_KV8_SEG_COST 8
+#endif
+constexpr int SEG_COST = QW_KV8_SEG_COST;
+
 struct Where { int s, h, t; };                       // sequence, kv head, tile of the group
 
-__host__ __device__ __forceinline__ int share_lo(const Kv8AttnParams &p, int cta) {
-    return (int)((int64_t)p.total_tiles * cta / p.n_cta);
-}
-// The CTA whose share holds tile T: the largest c with floor(total * c / n) <= T.
+// The CTA whose share holds tile T: the last one that starts at or before it.
 __host__ __device__ __forceinline__ int share_of(const Kv8AttnParams &p, int T) {
-    return (int)((((int64_t)T + 1) * p.n_cta - 1) / p.total_tiles);
+    int c = 0, e = p.n_cta - 1;
+    while (c < e) {
+        const int m = (c + e + 1) >> 1;
+        if (p.share[m] <= T) c = m; else e = m - 1;
+    }
+    return c;
 }
 __device__ __forceinline__ Where locate(const Kv8AttnParams &p, int T) {
     int s = 0, e = p.n_seq - 1;
@@ -316,7 +343,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1) kv8_attn_kernel(const __grid_co
 
     uint8_t *ring = smem + kg * NS * ENTRY;
     full += kg * NS; empty += kg * NS; meta += kg * NS;
-    const int lo = share_lo(p, blockIdx.x), hi = share_lo(p, blockIdx.x + 1);
+    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
     Where w = locate(p, lo);
     uint32_t E0 = 0;                                 // ring entries of this kg group before the current segment
 
@@ -680,6 +707,8 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
         for (int i = 0; i < KG * NS; i++) mbar_init(&full[i], 1);
         *abort_flag = 0;
         mbar_fence_init();
+        tma_prefetch_desc(&p.maps[0]);
+        tma_prefetch_desc(&p.maps[1]);
     }
     __syncthreads();
     pdl_wait();
@@ -687,10 +716,16 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
 
     uint8_t *ring = smem + warp * NS * ENTRY;
     full += warp * NS;
-    const int lo = share_lo(p, blockIdx.x), hi = share_lo(p, blockIdx.x + 1);
+    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
     Where w = locate(p, lo);
     uint32_t phase = 0;                              // of both slots: K in slot 0, V in slot 1
 
+    auto load = [&](const Kv8AttnSeq &sq, int row, int is_v) {       // lane 0
+        mbar_expect_tx(&full[is_v], ENTRY);
+        const CUtensorMap *map = &p.maps[is_v ? sq.vmap : sq.kmap];
+        tma_load_2d(ring + is_v * ENTRY, map, 0, row, &full[is_v]);
+        tma_load_2d(ring + is_v * ENTRY + BOX, map, 128, row, &full[is_v]);
+    };
     for (int T = lo; T < hi;) {
         const Kv8AttnSeq &sq = p.seq[w.s];
         const int seg_t0 = w.t, seg_n = min(sq.n_tiles - w.t, hi - T);
@@ -711,15 +746,9 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
                 win_e = (ek & 0xffff) | (ev << 16);
             }
         };
-        auto load = [&](int row, int is_v) {         // lane 0
-            mbar_expect_tx(&full[is_v], ENTRY);
-            const CUtensorMap *map = &p.maps[is_v ? sq.vmap : sq.kmap];
-            tma_load_2d(ring + is_v * ENTRY, map, 0, row, &full[is_v]);
-            tma_load_2d(ring + is_v * ENTRY + BOX, map, 128, row, &full[is_v]);
-        };
         if (nt > 0) {
             window(0);
-            if (lane == 0) { load(win_k, 0); load(win_v, 1); }
+            if (lane == 0) { load(sq, win_k, 0); load(sq, win_v, 1); }
         }
 
         // ---- Q: one warp per row, 8 dims per lane, scaled below 2^14 and put where the B fragments are read: step
@@ -819,7 +848,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
                 }
             }
             __syncwarp();
-            if (lane == 0 && i + 1 < nt) load(nk, 0);
+            if (lane == 0 && i + 1 < nt) load(sq, nk, 0);
 
             // ---- online softmax ----
             const float k0 = sc0 * pow2f(ek), k1 = sc1 * pow2f(ek), fv = (float)ev;
@@ -906,7 +935,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
                 }
             }
             __syncwarp();
-            if (lane == 0 && i + 1 < nt) load(nv, 1);
+            if (lane == 0 && i + 1 < nt) load(sq, nv, 1);
         }
 
         // ---- segment end: every warp puts its sums into its first slot, and all threads add them up ----
@@ -966,55 +995,75 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
         for (int i = 0; i < 4096; i++) __nanosleep(10000);
 }
 
-// Partials of a cut group: one block per (group, row); the four quarters of the block take every fourth partial.
-__global__ void __launch_bounds__(256) kv8_merge_kernel(const __grid_constant__ Kv8AttnParams p, int max_valid) {
+// Partials of a cut group: one block per (group, row).  Slices of 64 threads x four dims take every MG_SLICES-th
+// partial each, ten loads in flight, asked for before the weights are known: one trip to L2 for up to 40 partials
+// (four slices: many groups, few partials each) or 160 (sixteen: few groups, cut over most of the SMs).
+constexpr int MG_FLY = 10;
+template <int MG_SLICES>
+__global__ void __launch_bounds__(MG_SLICES * 64) kv8_merge_kernel(const __grid_constant__ Kv8AttnParams p, int max_valid) {
     __shared__ float w_s[256];
     __shared__ float red_s[2][8];
-    __shared__ __align__(16) float acc_s[3][256];
+    __shared__ __align__(16) float acc_s[MG_SLICES][256];
     pdl_launch_next();
-    pdl_wait();
     const int gi = blockIdx.x / max_valid, row = blockIdx.x - gi * max_valid;
     const int s = gi / p.kv_heads, h = gi - s * p.kv_heads;
     const Kv8AttnSeq &sq = p.seq[s];
-    if (row >= sq.rows * p.gqa) return;
     const int G0 = sq.cum_tiles + h * sq.n_tiles, c0 = share_of(p, G0), parts = share_of(p, G0 + sq.n_tiles - 1) - c0 + 1;
-    if (parts == 1) return;                               // written whole
+    pdl_wait();
+    if (row >= sq.rows * p.gqa || parts == 1) return;     // (a group of one part was written whole)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int slice = tid >> 6, d4 = (tid & 63) * 4;
     const size_t pi0 = (size_t)(c0 + gi) * p.slot_rows + row;
-    float mq = -INFINITY, lq = 0.0f;
-    if (tid < parts) {
-        const float2 st = *reinterpret_cast<const float2 *>(p.pstat + (pi0 + (size_t)tid * p.slot_rows) * 2);
-        mq = st.x; lq = st.y;
+    const float *base = p.pacc + pi0 * 256 + d4;
+    const size_t step = (size_t)p.slot_rows * 256;
+    float4 a[MG_FLY];
+#pragma unroll
+    for (int u = 0; u < MG_FLY; u++) {
+        const int q = slice + MG_SLICES * u;
+        a[u] = q < parts ? *reinterpret_cast<const float4 *>(base + (size_t)q * step) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    float m = warp_max(mq);
-    if (lane == 0) red_s[0][warp] = m;
+    float mq = -INFINITY, lq = 0.0f;
+    if (tid < 256) {                                      // (parts <= CTAs <= 256)
+        if (tid < parts) {
+            const float2 st = *reinterpret_cast<const float2 *>(p.pstat + (pi0 + (size_t)tid * p.slot_rows) * 2);
+            mq = st.x; lq = st.y;
+        }
+        const float m = warp_max(mq);
+        if (lane == 0) red_s[0][warp] = m;
+    }
     __syncthreads();
-    m = red_s[0][0];
+    float m = red_s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; i++) m = fmaxf(m, red_s[0][i]);
-    const float wq = mq == m ? 1.0f : ex2(mq - m);
-    w_s[tid] = wq;
-    const float d = warp_sum(tid < parts ? lq * wq : 0.0f);
-    if (lane == 0) red_s[1][warp] = d;
+    if (tid < 256) {
+        const float wq = mq == m ? 1.0f : ex2(mq - m);
+        w_s[tid] = wq;
+        const float d = warp_sum(tid < parts ? lq * wq : 0.0f);
+        if (lane == 0) red_s[1][warp] = d;
+    }
     __syncthreads();
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < MG_FLY; u++) {
+        const int q = slice + MG_SLICES * u;
+        const float f = q < parts ? w_s[q] : 0.0f;
+        acc.x = fmaf(a[u].x, f, acc.x); acc.y = fmaf(a[u].y, f, acc.y); acc.z = fmaf(a[u].z, f, acc.z); acc.w = fmaf(a[u].w, f, acc.w);
+    }
+    for (int q = slice + MG_SLICES * MG_FLY; q < parts; q += MG_SLICES) {
+        const float4 b = *reinterpret_cast<const float4 *>(base + (size_t)q * step);
+        const float f = w_s[q];
+        acc.x = fmaf(b.x, f, acc.x); acc.y = fmaf(b.y, f, acc.y); acc.z = fmaf(b.z, f, acc.z); acc.w = fmaf(b.w, f, acc.w);
+    }
+    *reinterpret_cast<float4 *>(&acc_s[slice][d4]) = acc;
+    __syncthreads();
+    if (slice > 0) return;
     float den = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) den += red_s[1][i];
-    const int quarter = tid >> 6, d4 = (tid & 63) * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int q = quarter; q < parts; q += 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(p.pacc + (pi0 + (size_t)q * p.slot_rows) * 256 + d4);
-        const float f = w_s[q];
-        acc.x += a.x * f; acc.y += a.y * f; acc.z += a.z * f; acc.w += a.w * f;
-    }
-    if (quarter > 0) *reinterpret_cast<float4 *>(&acc_s[quarter - 1][d4]) = acc;
-    __syncthreads();
-    if (quarter > 0) return;
 #pragma unroll
-    for (int i = 0; i < 3; i++) {
-        const float4 a = *reinterpret_cast<const float4 *>(&acc_s[i][d4]);
-        acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
+    for (int i = 1; i < MG_SLICES; i++) {
+        const float4 b = *reinterpret_cast<const float4 *>(&acc_s[i][d4]);
+        acc.x += b.x; acc.y += b.y; acc.z += b.z; acc.w += b.w;
     }
     const int r = row / p.gqa;
     const float inv = 1.0f / den;
@@ -1092,8 +1141,26 @@ void kv8_attn_plan(Kv8AttnParams &p) {
         valid = std::max(valid, s.rows * p.gqa);
     }
     p.total_tiles = cum;
-    p.n_cta = std::min(std::min(sm_count(), 256), cum);      // the merge reads one partial per thread of 256
+    p.n_cta = std::min(std::min(sm_count(), 256), cum);
     p.slot_rows = valid;
+    // Shares of equal cost: a share that begins a group pays that segment's first loads and its sum over the warps
+    // on top of its tiles, SEG_COST tile times.  So every group is given that many virtual tiles in front, the virtual
+    // line is cut evenly, and a cut among the virtual tiles moves to the group's first real one.
+    const int groups = p.n_seq * p.kv_heads;
+    const int64_t v_total = (int64_t)cum + (int64_t)SEG_COST * groups;
+    int s = 0, h = 0;
+    int64_t v0 = 0;                                          // virtual start of group (s, h)
+    int t0 = 0;                                              // its first real tile
+    for (int c = 0; c < p.n_cta; c++) {
+        const int64_t v = v_total * c / p.n_cta;
+        while (v >= v0 + SEG_COST + p.seq[s].n_tiles) {
+            v0 += SEG_COST + p.seq[s].n_tiles;
+            t0 += p.seq[s].n_tiles;
+            if (++h == p.kv_heads) { h = 0; s++; }
+        }
+        p.share[c] = t0 + (int)std::max<int64_t>(0, v - v0 - SEG_COST);
+    }
+    p.share[p.n_cta] = cum;
 }
 
 size_t kv8_attn_scratch_bytes(const Kv8AttnParams &p) {
@@ -1110,17 +1177,20 @@ void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scrat
     else
     if (f32) { if (mt <= 1) launch_attn_t<1, true>(s, p); else if (mt <= 2) launch_attn_t<2, true>(s, p); else launch_attn_t<4, true>(s, p); }
     else { if (mt <= 1) launch_attn_t<1, false>(s, p); else if (mt <= 2) launch_attn_t<2, false>(s, p); else launch_attn_t<4, false>(s, p); }
-    bool cut = false;
-    for (int i = 0; i < p.n_seq && !cut; i++)
-        for (int h = 0; h < p.kv_heads && !cut; h++) {
+    int parts = 0;                             // most partials of a cut group
+    for (int i = 0; i < p.n_seq; i++)
+        for (int h = 0; h < p.kv_heads; h++) {
             const int g0 = p.seq[i].cum_tiles + h * p.seq[i].n_tiles;
-            cut = share_of(p, g0) != share_of(p, g0 + p.seq[i].n_tiles - 1);
+            parts = std::max(parts, share_of(p, g0 + p.seq[i].n_tiles - 1) - share_of(p, g0));
         }
-    if (!cut) return;                          // every group was written whole
+    if (parts) parts++;
+    if (!parts) return;                        // every group was written whole
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
-    pdl_config(cfg, attr, dim3((unsigned)(p.n_seq * p.kv_heads * valid)), 256, 0, s);
-    cudaLaunchKernelEx(&cfg, kv8_merge_kernel, p, valid);
+    const bool few = parts <= 4 * MG_FLY;
+    pdl_config(cfg, attr, dim3((unsigned)(p.n_seq * p.kv_heads * valid)), few ? 256 : 1024, 0, s);
+    if (few) cudaLaunchKernelEx(&cfg, kv8_merge_kernel<4>, p, valid);
+    else cudaLaunchKernelEx(&cfg, kv8_merge_kernel<16>, p, valid);
     g_launches++;
 }
 

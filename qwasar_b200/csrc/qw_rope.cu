@@ -20,22 +20,22 @@ constexpr int ROPE_ITEMS = 4 * ROPE_THREADS;      // vectors a block takes befor
 template <typename T> struct Vec;                 // 16 bytes of T
 template <> struct Vec<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(float (&v)[4], const float *p) {
-        const float4 t = *reinterpret_cast<const float4 *>(p);
-        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    static __device__ __forceinline__ void unpack(float (&v)[4], uint4 t) {
+        v[0] = __uint_as_float(t.x); v[1] = __uint_as_float(t.y); v[2] = __uint_as_float(t.z); v[3] = __uint_as_float(t.w);
     }
-    static __device__ __forceinline__ void store(float *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
 };
 template <> struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(float (&v)[8], const __nv_bfloat16 *p) {
-        const uint4 t = *reinterpret_cast<const uint4 *>(p);
+    static __device__ __forceinline__ void unpack(float (&v)[8], uint4 t) {
         const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
     }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&v)[8]) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+        return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
     }
 };
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -51,6 +51,32 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeParams p, 
     pdl_launch_next();
     const int row = blockIdx.x, half = p.rotary_dim >> 1;
     const int head0 = blockIdx.y * heads_per_block, nh = min(heads_per_block, p.heads - head0);
+    const T *x = reinterpret_cast<const T *>(p.x) + (size_t)row * p.x_stride + (size_t)head0 * p.head_dim;
+    T *y = reinterpret_cast<T *>(p.y) + (size_t)row * p.y_stride + (size_t)head0 * p.head_dim;
+    const bool copy = (const void *)p.x != (const void *)p.y;     // in place: the dims that do not turn stay where they are
+    constexpr int N = VEC ? Vec<T>::N : 1;
+    // items of one head: rotations (N pairs each in the half layout, N / 2 or 1 in the interleaved one), then copies
+    const int per_rot = (INTER && VEC) ? N / 2 : N;
+    const int n_rot = half / per_rot, n_cp = copy ? (p.head_dim - p.rotary_dim) / N : 0;
+    const int per = n_rot + n_cp, total = nh * per;
+    // FLY vectors (half layout: pairs of vectors) of a thread are on their way at a time, the first ones under the angles
+    constexpr int FLY = 4;
+    uint4 a[FLY], b[FLY];
+    int off[FLY], idx[FLY];
+    auto fetch = [&](int it0) {
+#pragma unroll
+        for (int f = 0; f < FLY; f++) {
+            const int it = it0 + f * ROPE_THREADS;
+            const int h = it / per, i = it - h * per;
+            idx[f] = it < total ? i : -1;
+            off[f] = h * p.head_dim + (i < n_rot ? i * N : p.rotary_dim + (i - n_rot) * N);
+            if (it < total) {
+                a[f] = *reinterpret_cast<const uint4 *>(x + off[f]);
+                if (!INTER && i < n_rot) b[f] = *reinterpret_cast<const uint4 *>(x + off[f] + half);
+            }
+        }
+    };
+    if constexpr (VEC) fetch(threadIdx.x);
     const double pos = (double)p.pos[row];
     for (int j = threadIdx.x; j < half; j += ROPE_THREADS) {
         const double a = pos * (double)p.inv_freq[j];
@@ -62,48 +88,44 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeParams p, 
         cs[j] = make_float2(c * p.amp, s * p.amp);
     }
     __syncthreads();
-    const T *x = reinterpret_cast<const T *>(p.x) + (size_t)row * p.x_stride + (size_t)head0 * p.head_dim;
-    T *y = reinterpret_cast<T *>(p.y) + (size_t)row * p.y_stride + (size_t)head0 * p.head_dim;
-    const bool copy = (const void *)p.x != (const void *)p.y;     // in place: the dims that do not turn stay where they are
-    constexpr int N = VEC ? Vec<T>::N : 1;
-    // items of one head: rotations (N pairs each in the half layout, N / 2 or 1 in the interleaved one), then copies
-    const int per_rot = (INTER && VEC) ? N / 2 : N;
-    const int n_rot = half / per_rot, n_cp = copy ? (p.head_dim - p.rotary_dim) / N : 0;
-    const int per = n_rot + n_cp;
-    for (int it = threadIdx.x; it < nh * per; it += ROPE_THREADS) {
-        const int h = it / per, i = it - h * per;
-        const T *xh = x + (size_t)h * p.head_dim;
-        T *yh = y + (size_t)h * p.head_dim;
-        if constexpr (VEC) {
-            float a[N];
-            if (i >= n_rot) {
-                const int d = p.rotary_dim + (i - n_rot) * N;
-                *reinterpret_cast<uint4 *>(yh + d) = *reinterpret_cast<const uint4 *>(xh + d);
-            } else if constexpr (INTER) {
-                Vec<T>::load(a, xh + i * N);
+    if constexpr (VEC) {
+        for (int it0 = threadIdx.x; it0 < total; it0 += FLY * ROPE_THREADS) {
+            if (it0 != (int)threadIdx.x) fetch(it0);
 #pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const float2 t = cs[i * (N / 2) + e / 2];
-                    const float u = a[e], v = a[e + 1];
-                    a[e] = u * t.x - v * t.y;
-                    a[e + 1] = v * t.x + u * t.y;
-                }
-                Vec<T>::store(yh + i * N, a);
-            } else {
-                float b[N];
-                Vec<T>::load(a, xh + i * N);
-                Vec<T>::load(b, xh + half + i * N);
+            for (int f = 0; f < FLY; f++) {
+                if (idx[f] < 0) break;
+                T *o = y + off[f];
+                if (idx[f] >= n_rot) { *reinterpret_cast<uint4 *>(o) = a[f]; continue; }
+                float u[N];
+                Vec<T>::unpack(u, a[f]);
+                if constexpr (INTER) {
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float2 t = cs[i * N + e];
-                    const float u = a[e], v = b[e];
-                    a[e] = u * t.x - v * t.y;
-                    b[e] = v * t.x + u * t.y;
+                    for (int e = 0; e < N; e += 2) {
+                        const float2 t = cs[idx[f] * (N / 2) + e / 2];
+                        const float p0 = u[e], p1 = u[e + 1];
+                        u[e] = p0 * t.x - p1 * t.y;
+                        u[e + 1] = p1 * t.x + p0 * t.y;
+                    }
+                } else {
+                    float v[N];
+                    Vec<T>::unpack(v, b[f]);
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const float2 t = cs[idx[f] * N + e];
+                        const float p0 = u[e], p1 = v[e];
+                        u[e] = p0 * t.x - p1 * t.y;
+                        v[e] = p1 * t.x + p0 * t.y;
+                    }
+                    *reinterpret_cast<uint4 *>(o + half) = Vec<T>::pack(v);
                 }
-                Vec<T>::store(yh + i * N, a);
-                Vec<T>::store(yh + half + i * N, b);
+                *reinterpret_cast<uint4 *>(o) = Vec<T>::pack(u);
             }
-        } else {
+        }
+    } else {
+        for (int it = threadIdx.x; it < total; it += ROPE_THREADS) {
+            const int h = it / per, i = it - h * per;
+            const T *xh = x + (size_t)h * p.head_dim;
+            T *yh = y + (size_t)h * p.head_dim;
             if (i >= n_rot) {
                 const int d = p.rotary_dim + i - n_rot;
                 yh[d] = xh[d];
