@@ -265,7 +265,7 @@ struct Kv8AttnSeq {
     uint8_t kmap, vmap;
 };
 struct Kv8AttnParams {
-    CUtensorMap maps[QW_MAX_MAPS];     // code rows, boxes of 128 bytes x 32 rows, SWIZZLE_128B
+    CUtensorMap maps[QW_KV8_MAPS];     // code rows, boxes of 128 bytes x kv8_box_rows() rows, SWIZZLE_128B
     Kv8AttnSeq seq[QW_MAX_SEQ];
     int32_t n_seq, q_heads, kv_heads, gqa;
     int32_t total_tiles, n_cta, slot_rows;
@@ -275,11 +275,33 @@ struct Kv8AttnParams {
     float *pacc, *pstat;     // partials: [slot, slot_rows, 256] and [slot, slot_rows, 2]; slot = cta + group
     int *status;
 };
-// Query rows (rows * gqa) one sequence of a launch may have.
-inline int kv8_max_query_rows(int io) { return io == DT_F32 ? 32 : 64; }
+// Query rows (rows * gqa) one sequence of a launch may have, and the box height its kernel loads with: a decode step
+// takes whole tiles of 32 keys, more rows share a tile between two warps of 16 keys each.
+constexpr int KV8_MAX_QUERY_ROWS = 32;
+inline int kv8_box_rows(int query_rows) { return query_rows <= 8 ? 32 : 16; }
 void kv8_attn_plan(Kv8AttnParams &p);
 size_t kv8_attn_scratch_bytes(const Kv8AttnParams &p);
 void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scratch);
+
+// Many bf16 rows over an 8-bit cache on tcgen05 (qw_kv8_prefill.cu).
+struct Kv8PrefillParams {
+    CUtensorMap kmap, vmap;  // code rows, boxes of 128 bytes x 64 rows
+    // [rows][q_heads][256] bf16 tensors (gate: heads gate_stride apart), boxes of 64 dims x gqa heads x tile_rows rows
+    CUtensorMap qmap, omap, gmap;
+    Kv8Layer kc, vc;
+    __nv_bfloat16 *out;
+    const __nv_bfloat16 *gate;       // nullptr: no gate
+    int32_t gate_stride, gated;
+    int32_t rows, base_pos, q_heads, kv_heads, gqa;
+    int32_t tile_rows, n_q_tiles, splits;   // rows of the call per tile (128 / gqa), tiles, shares of the keys
+    int32_t box_bytes;       // 128 * gqa * tile_rows
+    float scale;
+    float *pacc, *pstat;     // splits > 1: per (tile, kv head, share) sums and (max, sum) per tile row
+    int *status;
+};
+int kv8_prefill_splits(int tiles, int steps, int sms);
+size_t kv8_prefill_scratch_bytes(const Kv8PrefillParams &p);
+void launch_kv8_prefill(cudaStream_t s, Kv8PrefillParams &p, void *scratch);
 
 int sm_count();
 

@@ -218,47 +218,33 @@ __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(T *__restrict__ ds
 // =======================================================================================
 // attention, few query rows: split over the keys
 // =======================================================================================
-// All (sequence, kv head) groups of a launch lie end to end as one line of 32-key tiles, cut into equal shares, one
-// per CTA (one CTA per SM); a share that crosses a group's end is taken as two segments.  Warp (mt, kg) of a CTA owns
-// 16 rows of the tensor op and every KG-th tile of the segment; the MT warps of one kg read the same tiles.
+// All (sequence, kv head) groups of a launch lie end to end as one line of 32-key tiles, cut into shares of equal
+// cost, one per CTA (one CTA per SM); a share that crosses a group's end is taken as two segments.  The tiles of a
+// segment are dealt to the CTA's warps, each of which keeps its own running maximum, sum and output; the warps are
+// added up through shared memory at the segment's end, the CTAs of a cut group by a second kernel.
 //
-// Rows.  Query row i = r * gqa + g of the group (all query heads of the kv head).  fp16 tensor ops, because an e4m3
-// code is an fp16 number exactly.  bf16 rows are exact in fp16 after scaling by a power of two; 16 of them fill a row
-// tile.  f32 rows are cut into a high and a low fp16 part (22 bits), eight rows to a tile: row i's high part in tensor
-// row i, its low part in tensor row i + 8 -- the two sums land in one thread, which adds them.  The softmax weights
-// are cut the same way.  (Weights run up to 2^14, not 1, so that the small ones of a long context stay above fp16's
-// smallest number: 2^-38 of the largest.)
+// The products are turned over: S^T = K Q^T and O^T = V^T P^T, so that the cache is the 16-row operand of the tensor
+// op and the query rows are its eight columns.  With Q as the 16-row operand half of every op of a decode step would
+// multiply padding, and the running output would take twice the registers.  Query row i = r * gqa + g of the group:
+// all query heads of the kv head, all rows of the call.
+//
+// Types.  fp16 tensor ops, because an e4m3 code is an fp16 number exactly.  bf16 rows are exact in fp16 after scaling
+// by a power of two.  f32 rows are cut into a high and a low fp16 part (22 bits) that go through the same accumulators
+// one after the other; so are the softmax weights.  (Weights run up to 2^14, not 1, so that the small ones of a long
+// context stay above fp16's smallest number: 2^-38 of the largest.)
 //
 // Exponents.  A tile of 32 keys has one exponent for K and one for V.  With t = scale * log2(e) * 2^ek * (q . ck) + ev
 // and m the running maximum of t, w = 2^(t - m) weighs the V CODES: o = sum w cv, and the denominator is
 // l = sum w 2^-ev.  Both see each element once, as it lies in the cache.
 //
-// Loads.  Each kg group has a ring of 8 KB slots (K or V of one 32-key tile: two boxes of 128 bytes x 32 rows,
-// SWIZZLE_128B), filled by its first warp as the slots fall free; there is no producer warp, since eight consumer
-// warps with 255 registers each take the whole register file.
-constexpr int AT_THREADS = 256, AT_WARPS = 8;
+// Fragments.  A lane reads 16 bytes of one key (16 dims: four k-steps) or 16 dims of one key of V; keys are dealt to
+// lanes so that the eight lanes of a shared-memory phase meet eight different bank groups of the SWIZZLE_128B boxes.
+// The two keys of a V register are interleaved byte by byte before they are widened.  The weights come out with a key
+// per lane group and are wanted with a query row there: movmatrix turns an 8 x 8 block.
 constexpr int TILE = 32;
 constexpr int ENTRY = TILE * 256;                    // K or V codes of a tile
 constexpr int BOX = TILE * 128;
-constexpr int RING = 24;                             // slots of a CTA
-constexpr int OFF_Q = RING * ENTRY;
 constexpr float W_SHIFT = 14.0f;
-
-template <int MT>
-struct AtCfg {
-    static constexpr int KG = AT_WARPS / MT;
-    static constexpr int NS = RING / KG;                         // slots of one kg group
-    static constexpr int LAG = MT > 1 ? 2 : 0;                   // entries the loader lets the other warps fall behind
-    static constexpr int OFF_M = OFF_Q + MT * 8192;              // [KG][MT * 16]
-    static constexpr int OFF_L = OFF_M + AT_WARPS * 64;
-    static constexpr int OFF_QE = OFF_L + AT_WARPS * 64;         // [MT * 16] row exponents
-    static constexpr int OFF_META = OFF_QE + MT * 64;            // [RING] exponent of the slot's tile
-    static constexpr int OFF_BAR = OFF_META + RING * 4;          // full[RING], empty[RING], abort
-    static constexpr int SMEM = OFF_BAR + 2 * RING * 8 + 16;
-    static_assert(OFF_BAR % 8 == 0 && SMEM <= 232448, "exceeds the 227 KB a CTA may use");
-    static_assert(AT_WARPS * 16384 <= RING * ENTRY, "the warps' sums do not fit the ring");
-};
-
 #ifndef QW_KV8_SEG_COST
 #define QW_KV8_SEG_COST 8
 #endif
@@ -293,8 +279,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void bar_all() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
 __device__ __forceinline__ float load1(const void *g, size_t i, int io) {
     return io == DT_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(g)[i]) : reinterpret_cast<const float *>(g)[i];
 }
@@ -311,370 +295,17 @@ __device__ __forceinline__ void store_out(const Kv8AttnParams &p, const Kv8AttnS
         *reinterpret_cast<float4 *>(reinterpret_cast<float *>(sq.out) + rh * 256 + d4) = o;
 }
 
-template <int MT, bool F32>
-__global__ void __launch_bounds__(AT_THREADS, 1) kv8_attn_kernel(const __grid_constant__ Kv8AttnParams p) {
-    using Cfg = AtCfg<MT>;
-    constexpr int KG = Cfg::KG, NS = Cfg::NS, LAG = Cfg::LAG;
-    constexpr int RT = F32 ? 8 : 16;                 // query rows of a row tile
-    extern __shared__ __align__(1024) uint8_t smem[];
-    float *sm_m = reinterpret_cast<float *>(smem + Cfg::OFF_M);
-    float *sm_l = reinterpret_cast<float *>(smem + Cfg::OFF_L);
-    int *sm_qe = reinterpret_cast<int *>(smem + Cfg::OFF_QE);
-    int *meta = reinterpret_cast<int *>(smem + Cfg::OFF_META);
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::OFF_BAR);
-    uint64_t *empty = full + RING;
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(empty + RING);
-
-    if (smem_u32(smem) & 1023u) {                    // swizzled boxes need 1024-byte alignment
-        if (threadIdx.x == 0) report(p.status, QW_ST_BAD_SMEM);
-        return;
-    }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int mt = warp % MT, kg = warp / MT;
-    const int g = lane >> 2, t = lane & 3;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < RING; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], MT); }
-        *abort_flag = 0;
-        mbar_fence_init();
-    }
-    __syncthreads();
-    pdl_wait();
-    pdl_launch_next();
-
-    uint8_t *ring = smem + kg * NS * ENTRY;
-    full += kg * NS; empty += kg * NS; meta += kg * NS;
-    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
-    Where w = locate(p, lo);
-    uint32_t E0 = 0;                                 // ring entries of this kg group before the current segment
-
-    for (int T = lo; T < hi;) {
-        const Kv8AttnSeq &sq = p.seq[w.s];
-        const int seg_t0 = w.t, seg_n = min(sq.n_tiles - w.t, hi - T);
-        const int valid = sq.rows * p.gqa, head0 = w.h * p.gqa;
-        const int n_keys = sq.base_pos + sq.rows;
-        const int nt = kg < seg_n ? (seg_n - kg + KG - 1) / KG : 0;      // this warp's tiles
-        const uint32_t E1 = E0 + 2 * nt;
-
-        // ---- loads: entry E of the group is K (even) or V (odd) of its tile (E - E0) / 2 ----
-        int win_k = 0, win_v = 0, win_e = 0;         // code rows and exponents of 32 tiles, one per lane
-        auto window = [&](int i0) {
-            const int i = i0 + lane;
-            if (i < nt) {
-                const int key = (seg_t0 + kg + i * KG) * TILE;
-                const int64_t kr = code_row(sq.kc, w.h, key), vr = code_row(sq.vc, w.h, key);
-                if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
-                win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
-                const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key / BLK]);
-                const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key / BLK]);
-                win_e = (ek & 0xffff) | (ev << 16);
-            }
-        };
-        auto load = [&](uint32_t E) {                // the whole warp mt == 0
-            const int i = (int)(E - E0) >> 1, is_v = (int)(E - E0) & 1;
-            if (!is_v && (i & 31) == 0) window(i);
-            const int row = __shfl_sync(0xffffffffu, is_v ? win_v : win_k, i & 31);
-            const int ex = __shfl_sync(0xffffffffu, win_e, i & 31);
-            if (lane == 0) {
-                const uint32_t slot = E % NS;
-                if (MT > 1 && E >= NS) mbar_wait(&empty[slot], (E / NS - 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
-                meta[slot] = is_v ? ex >> 16 : (int)(int16_t)(ex & 0xffff);
-                mbar_expect_tx(&full[slot], ENTRY);
-                const CUtensorMap *map = &p.maps[is_v ? sq.vmap : sq.kmap];
-                tma_load_2d(ring + slot * ENTRY, map, 0, row, &full[slot]);
-                tma_load_2d(ring + slot * ENTRY + BOX, map, 128, row, &full[slot]);
-            }
-            __syncwarp();
-        };
-        // a finished entry's slot is handed back; the loader refills the slot that fell free LAG entries ago
-        auto done = [&](uint32_t E) {
-            __syncwarp();
-            if (MT > 1 && lane == 0) mbar_arrive(&empty[E % NS]);
-            if (mt == 0) {
-                const uint32_t nx = E + NS - LAG;
-                if (E >= E0 + LAG && nx < E1) load(nx);
-            }
-        };
-        if (mt == 0)
-            for (uint32_t E = E0; E < E1 && E < E0 + NS; E++) load(E);
-
-        // ---- Q: one warp per row, 8 dims per lane, scaled to [2^13, 2^14) and put where the tensor op's A fragments
-        // are read: step 4 q + i of a row tile takes dims 64 q + 16 t + 4 i + {0, 1 | 2, 3} of lane (g, t) ----
-        for (int row = warp; row < MT * RT; row += AT_WARPS) {
-            float x[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = 0.0f;
-            if (row < valid) {
-                const int r = row / p.gqa, hh = row - r * p.gqa;
-                const size_t at = ((size_t)r * p.q_heads + head0 + hh) * 256 + lane * 8;
-                if constexpr (F32) {
-                    const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at);
-                    const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at + 4);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                } else {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(sq.q) + at);
-                    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
-                }
-            }
-            float mx = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
-            mx = warp_max(mx);
-            // row exponent: x * 2^-qe is below 2^14 (kept where 2^-qe and 2^qe are normal numbers)
-            const int qe = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 13, -100), 100);
-            const float f = pow2f(-qe);
-            if (lane == 0) sm_qe[row] = qe;
-            const int q = lane >> 3, tt = (lane >> 1) & 3, i0 = (lane & 1) * 2;
-            const int tile = row / RT, rr = row % RT;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                uint32_t *fr = reinterpret_cast<uint32_t *>(smem + OFF_Q) + (((size_t)tile * 16 + q * 4 + i0 + i) * 32 + (rr & 7) * 4 + tt) * 4;
-                const float a = x[4 * i] * f, b = x[4 * i + 1] * f, c = x[4 * i + 2] * f, d = x[4 * i + 3] * f;
-                const uint32_t ab = pack_f16(a, b), cd = pack_f16(c, d);
-                if constexpr (F32) {
-                    const float2 hab = h2f2(ab), hcd = h2f2(cd);
-                    *reinterpret_cast<uint4 *>(fr) = make_uint4(ab, pack_f16(a - hab.x, b - hab.y), cd, pack_f16(c - hcd.x, d - hcd.y));
-                } else {
-                    fr[rr >> 3] = ab; fr[2 + (rr >> 3)] = cd;
-                }
-            }
-        }
-        bar_all();
-
-        float o[32][4];
-#pragma unroll
-        for (int n = 0; n < 32; n++) { o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f; }
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        const int row0 = mt * RT + g, row1 = row0 + 8;                   // (f32: only row0, its low part in tensor row 8 + g)
-        const int lim0 = row0 < valid ? sq.base_pos + row0 / p.gqa : n_keys - 1;
-        const int lim1 = F32 ? lim0 : row1 < valid ? sq.base_pos + row1 / p.gqa : n_keys - 1;
-        const float sc0 = p.scale * LOG2E * pow2f(sm_qe[row0]);
-        const float sc1 = F32 ? sc0 : p.scale * LOG2E * pow2f(sm_qe[row1]);
-        const uint32_t q_base = smem_u32(smem + OFF_Q) + mt * 8192 + lane * 16;
-
-        for (int i = 0; i < nt; i++) {
-            const int key0 = (seg_t0 + kg + i * KG) * TILE;
-            const uint32_t EK = E0 + 2 * i, EV = EK + 1;
-            // ---- S = Q K^T: column n of the tensor op is token n ^ 4 (n & 1) of its group of eight, so that the eight
-            // lanes of a shared-memory phase meet eight different bank groups ----
-            float s[4][4];
-#pragma unroll
-            for (int n = 0; n < 4; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            mbar_wait(&full[EK % NS], (EK / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-            const int ek = meta[EK % NS];
-            {
-                const uint32_t tok = (uint32_t)(g ^ ((g & 1) << 2));
-                const uint32_t kb = smem_u32(ring + (EK % NS) * ENTRY) + tok * 128;
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t kw[4][4];
-#pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(kw[n][0]), "=r"(kw[n][1]), "=r"(kw[n][2]), "=r"(kw[n][3])
-                                     : "r"(kb + (q >> 1) * BOX + n * 1024 + ((((uint32_t)(4 * (q & 1) + t)) ^ tok) << 4)));
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t a0, a1, a2, a3;
-                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3) : "r"(q_base + (q * 4 + k) * 512));
-#pragma unroll
-                        for (int n = 0; n < 4; n++) mma_f16(s[n], a0, a1, a2, a3, f16x2_lo(kw[n][k]), f16x2_hi(kw[n][k]));
-                    }
-                }
-            }
-            done(EK);
-            mbar_wait(&full[EV % NS], (EV / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-            const int ev = meta[EV % NS];
-
-            // ---- online softmax ----
-            const float k0 = sc0 * pow2f(ek), k1 = sc1 * pow2f(ek), fv = (float)ev;
-            if constexpr (F32) {
-#pragma unroll
-                for (int n = 0; n < 4; n++) { s[n][0] += s[n][2]; s[n][1] += s[n][3]; }
-            }
-            constexpr int ROWS = F32 ? 2 : 4;         // values of a thread: two columns of one or two rows
-#pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int c = 0; c < ROWS; c++) s[n][c] = fmaf(s[n][c], c < 2 ? k0 : k1, fv);
-            if (key0 + TILE > sq.base_pos + 1) {
-#pragma unroll
-                for (int n = 0; n < 4; n++)
-#pragma unroll
-                    for (int c = 0; c < ROWS; c++) {
-                        const int key = key0 + n * 8 + ((c & 1) ? ((2 * t + 1) ^ 4) : 2 * t);
-                        if (key > (c < 2 ? lim0 : lim1)) s[n][c] = -INFINITY;
-                    }
-            }
-            float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
-                if (!F32) x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
-            }
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-            if (!F32) {
-                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-            }
-            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-                const float f0 = m0 == n0 ? 1.0f : ex2(m0 - n0), f1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
-                l0 *= f0; l1 *= f1;
-#pragma unroll
-                for (int n = 0; n < 32; n++) { o[n][0] *= f0; o[n][1] *= f0; o[n][2] *= F32 ? f0 : f1; o[n][3] *= F32 ? f0 : f1; }
-                m0 = n0; m1 = n1;
-            }
-            const float b0 = (m0 == -INFINITY ? 0.0f : m0) - W_SHIFT, b1 = (m1 == -INFINITY ? 0.0f : m1) - W_SHIFT;
-            uint32_t pa[2][4];
-            float a0 = 0.0f, a1 = 0.0f;
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const float w0 = ex2(s[n][0] - b0), w1 = ex2(s[n][1] - b0);
-                a0 += w0 + w1;
-                const uint32_t hi = pack_f16(w0, w1);
-                pa[n >> 1][(n & 1) * 2] = hi;
-                if constexpr (F32) {
-                    const float2 h = h2f2(hi);
-                    pa[n >> 1][(n & 1) * 2 + 1] = pack_f16(w0 - h.x, w1 - h.y);
-                } else {
-                    const float w2 = ex2(s[n][2] - b1), w3 = ex2(s[n][3] - b1);
-                    a1 += w2 + w3;
-                    pa[n >> 1][(n & 1) * 2 + 1] = pack_f16(w2, w3);
-                }
-            }
-            const float iv = pow2f(-ev);
-            l0 = fmaf(a0, iv, l0); l1 = fmaf(a1, iv, l1);
-
-            // ---- O += W V: column g of tile (x, d) is dim 128 x + 16 g + d; the two tokens of a B register are
-            // interleaved byte by byte before they are widened ----
-            const uint32_t vb = smem_u32(ring + (EV % NS) * ENTRY);
-            const bool ragged = key0 + TILE > n_keys;     // rows past the last key may hold anything
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                const uint32_t ta = 16 * kk + 2 * t, tb = 16 * kk + ((2 * t + 1) ^ 4);
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    uint32_t v[4][4];                     // tokens ta, tb, ta + 8, tb + 8
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t tok = ((c & 1) ? tb : ta) + (c >> 1) * 8;
-                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[c][0]), "=r"(v[c][1]), "=r"(v[c][2]), "=r"(v[c][3])
-                                     : "r"(vb + x * BOX + tok * 128 + (((uint32_t)g ^ (tok & 7)) << 4)));
-                        if (ragged && key0 + (int)tok >= n_keys) v[c][0] = v[c][1] = v[c][2] = v[c][3] = 0;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140), p1 = __byte_perm(v[0][k], v[1][k], 0x7362);
-                        const uint32_t r0 = __byte_perm(v[2][k], v[3][k], 0x5140), r1 = __byte_perm(v[2][k], v[3][k], 0x7362);
-                        const int n = x * 16 + k * 4;
-                        mma_f16(o[n], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_lo(p0), f16x2_lo(r0));
-                        mma_f16(o[n + 1], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_hi(p0), f16x2_hi(r0));
-                        mma_f16(o[n + 2], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_lo(p1), f16x2_lo(r1));
-                        mma_f16(o[n + 3], pa[kk][0], pa[kk][1], pa[kk][2], pa[kk][3], f16x2_hi(p1), f16x2_hi(r1));
-                    }
-                }
-            }
-            done(EV);
-        }
-        E0 = E1;
-
-        // ---- segment end: the KG warps of a row tile put their sums side by side into the ring (idle: every entry
-        // was consumed), and all threads add them up ----
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if (t == 0) {
-            sm_m[kg * MT * RT + row0] = m0; sm_l[kg * MT * RT + row0] = l0;
-            if (!F32) { sm_m[kg * MT * RT + row1] = m1; sm_l[kg * MT * RT + row1] = l1; }
-        }
-        bar_all();
-        float M0 = -INFINITY, M1 = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < KG; k++) {
-            M0 = fmaxf(M0, sm_m[k * MT * RT + row0]);
-            if (!F32) M1 = fmaxf(M1, sm_m[k * MT * RT + row1]);
-        }
-        {
-            const float f0 = m0 == M0 ? 1.0f : ex2(m0 - M0), f1 = m1 == M1 ? 1.0f : ex2(m1 - M1);
-            // the thread's dims of a row: 128 x + 32 t + [0, 16) and + [16, 32), as 16-byte pieces; piece c of a row
-            // sits at c ^ (t + 4 (row & 1)), which spreads a phase's eight lanes over the banks
-            float *own = reinterpret_cast<float *>(smem) + (size_t)warp * 4096;
-            const uint32_t sw = (uint32_t)(t + ((g & 1) << 2));
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        const int n = x * 16 + d * 4;
-                        const uint32_t piece = ((uint32_t)(x * 32 + t * 8 + c * 4 + d)) ^ sw;
-                        float4 a = make_float4(o[n][c], o[n + 1][c], o[n + 2][c], o[n + 3][c]);
-                        const float4 b = make_float4(o[n][2 + c], o[n + 1][2 + c], o[n + 2][2 + c], o[n + 3][2 + c]);
-                        if constexpr (F32) {
-                            a = make_float4((a.x + b.x) * f0, (a.y + b.y) * f0, (a.z + b.z) * f0, (a.w + b.w) * f0);
-                            *reinterpret_cast<float4 *>(own + g * 256 + piece * 4) = a;
-                        } else {
-                            *reinterpret_cast<float4 *>(own + g * 256 + piece * 4) = make_float4(a.x * f0, a.y * f0, a.z * f0, a.w * f0);
-                            *reinterpret_cast<float4 *>(own + (g + 8) * 256 + piece * 4) = make_float4(b.x * f1, b.y * f1, b.z * f1, b.w * f1);
-                        }
-                    }
-        }
-        bar_all();
-        const bool whole = seg_t0 == 0 && seg_n == sq.n_tiles;
-        const size_t slot = (size_t)blockIdx.x + (size_t)w.s * p.kv_heads + w.h;
-        for (int idx = threadIdx.x; idx < valid * 64; idx += AT_THREADS) {
-            const int row = idx >> 6, pc = idx & 63;
-            const int tile = row / RT, rr = row % RT;
-            const uint32_t piece = (uint32_t)pc ^ (uint32_t)(((pc >> 3) & 3) + ((rr & 1) << 2));
-            float M = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < KG; k++) M = fmaxf(M, sm_m[k * MT * RT + row]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float L = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KG; k++) {
-                const float mk = sm_m[k * MT * RT + row];
-                L += sm_l[k * MT * RT + row] * (mk == M ? 1.0f : ex2(mk - M));
-                const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + (size_t)(k * MT + tile) * 4096 + rr * 256 + piece * 4);
-                acc.x += a.x; acc.y += a.y; acc.z += a.z; acc.w += a.w;
-            }
-            if (whole) {
-                const int r = row / p.gqa;
-                const size_t rh = (size_t)r * p.q_heads + head0 + (row - r * p.gqa);
-                const float inv = 1.0f / L;
-                store_out(p, sq, rh, pc * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-            } else {
-                const size_t pi = slot * p.slot_rows + row;
-                *reinterpret_cast<float4 *>(p.pacc + pi * 256 + pc * 4) = acc;
-                if (pc == 0) *reinterpret_cast<float2 *>(p.pstat + pi * 2) = make_float2(M, L);
-            }
-        }
-        T += seg_n;
-        w.t = 0;                                          // the next segment, if any, begins the next group
-        if (++w.h == p.kv_heads) { w.h = 0; w.s++; }
-        fence_proxy_async();                              // the ring goes back to the copy engine
-        bar_all();
-    }
-    if (*abort_flag)                                      // a wait gave up: copies of this CTA may still be under way
-        for (int i = 0; i < 4096; i++) __nanosleep(10000);
-}
-
 // =======================================================================================
 // attention, up to eight query rows (a decode step)
 // =======================================================================================
-// The same line of tiles, shares and rings, with the products turned over: S^T = K Q^T and O^T = V^T P^T, so that the
-// cache is the 16-row operand of the tensor op and the query rows its eight columns.  With Q as the 16-row operand
-// half of every tensor op would multiply padding, and the running output would take 128 registers a thread instead of
-// 64; at 64, twelve warps fit an SM instead of eight, and the kernel stops waiting on its own instruction latency.
-// f32 rows put their high and low parts through the same accumulators one after the other.
-// The weights come out with a key per lane group and are wanted with a query row there: movmatrix turns an 8 x 8 block.
+// A warp takes whole tiles: K in one 8 KB slot of its own, V in another, each refilled as soon as it is read, so that
+// the other's load runs under its arithmetic.  The running output is 64 registers a thread; twelve warps fit an SM.
 constexpr int D_WARPS = 12, D_THREADS = D_WARPS * 32, D_NS = 2;
 constexpr int D_OFF_Q = D_WARPS * D_NS * ENTRY;
 constexpr int D_OFF_M = D_OFF_Q + 8192;                   // [warp][8]
 constexpr int D_OFF_L = D_OFF_M + D_WARPS * 32;
-constexpr int D_OFF_QE = D_OFF_L + D_WARPS * 32;          // [8]
-constexpr int D_OFF_BAR = D_OFF_QE + 32;                  // full[warps * slots], abort
+constexpr int D_OFF_SC = D_OFF_L + D_WARPS * 32;          // [8]
+constexpr int D_OFF_BAR = D_OFF_SC + 32;                  // full[warps * slots], abort
 constexpr int D_SMEM = D_OFF_BAR + D_WARPS * D_NS * 8 + 16;
 static_assert(D_SMEM <= 232448, "exceeds the 227 KB a CTA may use");
 
@@ -687,13 +318,58 @@ __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
 }
 
+// One warp stages query row `row`: 8 dims per lane, scaled below 2^14 and put where the B fragments are read: step
+// 4 q + i takes dims 64 q + 16 t + 4 i + {0, 1 | 2, 3} of row g in lane (g, t).  `frag`: the row's tile of eight
+// (8 steps-pairs x 32 lanes x 16 bytes; f32: 16 steps, high and low parts).  sc: scale * log2(e) * the row's 2^qe.
+template <bool F32>
+__device__ __forceinline__ void stage_q(const Kv8AttnParams &p, const Kv8AttnSeq &sq, int head0, int valid, int row, int lane, uint8_t *frags, float *sc) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = 0.0f;
+    if (row < valid) {
+        const int r = row / p.gqa, hh = row - r * p.gqa;
+        const size_t at = ((size_t)r * p.q_heads + head0 + hh) * 256 + lane * 8;
+        if constexpr (F32) {
+            const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at);
+            const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at + 4);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(sq.q) + at);
+            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
+        }
+    }
+    float mx = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
+    mx = warp_max(mx);
+    const int qe = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 13, -100), 100);
+    const float f = pow2f(-qe);
+    if (lane == 0) *sc = p.scale * LOG2E * pow2f(qe);
+    uint32_t hp[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) { x[2 * k] *= f; x[2 * k + 1] *= f; hp[k] = pack_f16(x[2 * k], x[2 * k + 1]); }
+    const int q = lane >> 3, at = (row & 7) * 4 + ((lane >> 1) & 3);
+    uint4 *fr = reinterpret_cast<uint4 *>(frags) + (row >> 3) * (F32 ? 512 : 256);
+    if constexpr (F32) {
+        uint32_t lp[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) { const float2 h = h2f2(hp[k]); lp[k] = pack_f16(x[2 * k] - h.x, x[2 * k + 1] - h.y); }
+        fr[(q * 4 + (lane & 1) * 2) * 32 + at] = make_uint4(hp[0], hp[1], lp[0], lp[1]);
+        fr[(q * 4 + (lane & 1) * 2 + 1) * 32 + at] = make_uint4(hp[2], hp[3], lp[2], lp[3]);
+    } else {
+        fr[(q * 2 + (lane & 1)) * 32 + at] = make_uint4(hp[0], hp[1], hp[2], hp[3]);
+    }
+}
+
 template <bool F32>
 __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_constant__ Kv8AttnParams p) {
     constexpr int KG = D_WARPS, NS = D_NS;
     extern __shared__ __align__(1024) uint8_t smem[];
     float *sm_m = reinterpret_cast<float *>(smem + D_OFF_M);
     float *sm_l = reinterpret_cast<float *>(smem + D_OFF_L);
-    int *sm_qe = reinterpret_cast<int *>(smem + D_OFF_QE);
+    float *sm_sc = reinterpret_cast<float *>(smem + D_OFF_SC);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + D_OFF_BAR);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(full + KG * NS);
 
@@ -751,48 +427,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
             if (lane == 0) { load(sq, win_k, 0); load(sq, win_v, 1); }
         }
 
-        // ---- Q: one warp per row, 8 dims per lane, scaled below 2^14 and put where the B fragments are read: step
-        // 4 q + i takes dims 64 q + 16 t + 4 i + {0, 1 | 2, 3} of row g in lane (g, t) ----
-        for (int row = warp; row < 8; row += D_WARPS) {
-            float x[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = 0.0f;
-            if (row < valid) {
-                const int r = row / p.gqa, hh = row - r * p.gqa;
-                const size_t at = ((size_t)r * p.q_heads + head0 + hh) * 256 + lane * 8;
-                if constexpr (F32) {
-                    const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at);
-                    const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at + 4);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-                } else {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(sq.q) + at);
-                    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
-                }
-            }
-            float mx = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(x[k]));
-            mx = warp_max(mx);
-            const int qe = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 13, -100), 100);
-            const float f = pow2f(-qe);
-            if (lane == 0) sm_qe[row] = qe;
-            uint32_t hp[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) { x[2 * k] *= f; x[2 * k + 1] *= f; hp[k] = pack_f16(x[2 * k], x[2 * k + 1]); }
-            const int q = lane >> 3, tt = (lane >> 1) & 3;
-            if constexpr (F32) {
-                uint32_t lp[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) { const float2 h = h2f2(hp[k]); lp[k] = pack_f16(x[2 * k] - h.x, x[2 * k + 1] - h.y); }
-                uint4 *fr = reinterpret_cast<uint4 *>(smem + D_OFF_Q) + (q * 4 + (lane & 1) * 2) * 32 + row * 4 + tt;
-                fr[0] = make_uint4(hp[0], hp[1], lp[0], lp[1]);
-                fr[32] = make_uint4(hp[2], hp[3], lp[2], lp[3]);
-            } else {
-                reinterpret_cast<uint4 *>(smem + D_OFF_Q)[(q * 2 + (lane & 1)) * 32 + row * 4 + tt] = make_uint4(hp[0], hp[1], hp[2], hp[3]);
-            }
-        }
+        if (warp < 8) stage_q<F32>(p, sq, head0, valid, warp, lane, smem + D_OFF_Q, sm_sc + warp);
         __syncthreads();
 
         float o[16][4];
@@ -803,7 +438,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
         const int lim0 = row0 < valid ? sq.base_pos + row0 / p.gqa : n_keys - 1;
         const int lim1 = row1 < valid ? sq.base_pos + row1 / p.gqa : n_keys - 1;
-        const float sc0 = p.scale * LOG2E * pow2f(sm_qe[row0]), sc1 = p.scale * LOG2E * pow2f(sm_qe[row1]);
+        const float sc0 = sm_sc[row0], sc1 = sm_sc[row1];
         const uint32_t q_base = smem_u32(smem + D_OFF_Q) + lane * 16;
         const uint32_t tok = (uint32_t)(g ^ ((g & 1) << 2));         // this lane group's key of a block of eight
         const uint32_t k_base = smem_u32(ring) + tok * 128, v_base = smem_u32(ring + ENTRY);
@@ -995,6 +630,363 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
         for (int i = 0; i < 4096; i++) __nanosleep(10000);
 }
 
+// =======================================================================================
+// attention, 9 to 32 query rows (a verify step)
+// =======================================================================================
+// NT tiles of eight query rows.  Two warps share a tile of 32 keys: each scores 16 of its keys against all rows (the K
+// codes are widened once, however many rows there are) and each takes 128 dims of V for all 32 keys.  What they swap is
+// the weights, through shared memory, one barrier of the pair per tile: each weighs its keys against its own running
+// maximum, a whole number, so that the other can bring the weights to the common maximum by an exact power of two.
+template <int NT, bool F32>
+struct VfCfg {
+    static constexpr int WARPS = NT == 4 ? 8 : 12, PAIRS = WARPS / 2, THREADS = WARPS * 32;
+    static constexpr int NS = NT == 4 ? 4 : 3;                  // 4 KB slots of a warp: its part of K or V of a tile
+    static constexpr int PX = NT * 32 * (F32 ? 16 : 8);         // weights of one warp's keys, as B fragments
+    static constexpr int OFF_Q = WARPS * NS * 4096;
+    static constexpr int OFF_PX = OFF_Q + NT * (F32 ? 8192 : 4096);       // [pair][tile parity][half]
+    static constexpr int OFF_MX = OFF_PX + PAIRS * 4 * PX;      // [pair][tile parity][half][NT * 8]
+    static constexpr int OFF_M = OFF_MX + PAIRS * 4 * NT * 32;  // [warp][NT * 8]
+    static constexpr int OFF_L = OFF_M + WARPS * NT * 32;
+    static constexpr int OFF_SC = OFF_L + WARPS * NT * 32;      // [NT * 8]
+    static constexpr int OFF_LIM = OFF_SC + NT * 32;            // [NT * 8] last key of a row
+    static constexpr int OFF_BAR = OFF_LIM + NT * 32;           // full[warp][slot], abort
+    static constexpr int SMEM = OFF_BAR + WARPS * NS * 8 + 16;
+    static_assert(SMEM <= 232448, "exceeds the 227 KB a CTA may use");
+    static_assert(NT <= NS, "a warp's sums do not fit its slots");
+};
+
+template <int NT, bool F32>
+__global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(const __grid_constant__ Kv8AttnParams p) {
+    using Cfg = VfCfg<NT, F32>;
+    constexpr int NS = Cfg::NS, PAIRS = Cfg::PAIRS, ROWS = NT * 8;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    float *sm_m = reinterpret_cast<float *>(smem + Cfg::OFF_M);
+    float *sm_l = reinterpret_cast<float *>(smem + Cfg::OFF_L);
+    float *sm_sc = reinterpret_cast<float *>(smem + Cfg::OFF_SC);
+    int *sm_lim = reinterpret_cast<int *>(smem + Cfg::OFF_LIM);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::OFF_BAR);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(full + Cfg::WARPS * NS);
+
+    if (smem_u32(smem) & 1023u) {                    // swizzled boxes need 1024-byte alignment
+        if (threadIdx.x == 0) report(p.status, QW_ST_BAD_SMEM);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pair = warp >> 1, half = warp & 1;
+    const int g = lane >> 2, t = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < Cfg::WARPS * NS; i++) mbar_init(&full[i], 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&p.maps[0]);
+        tma_prefetch_desc(&p.maps[1]);
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_launch_next();
+
+    uint8_t *ring = smem + warp * NS * 4096;
+    full += warp * NS;
+    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
+    Where w = locate(p, lo);
+    uint32_t E0 = 0;                                 // ring entries of this warp before the current segment
+
+    for (int T = lo; T < hi;) {
+        const Kv8AttnSeq &sq = p.seq[w.s];
+        const int seg_t0 = w.t, seg_n = min(sq.n_tiles - w.t, hi - T);
+        const int valid = sq.rows * p.gqa, head0 = w.h * p.gqa;
+        const int n_keys = sq.base_pos + sq.rows;
+        const int nt = pair < seg_n ? (seg_n - pair + PAIRS - 1) / PAIRS : 0;      // this pair's tiles
+        const uint32_t E1 = E0 + 2 * nt;
+
+        int win_k = 0, win_v = 0, win_e = 0;         // code rows and exponents of 32 tiles, one per lane
+        auto window = [&](int i0) {
+            const int i = i0 + lane;
+            if (i < nt) {
+                const int key = (seg_t0 + pair + i * PAIRS) * TILE;
+                const int64_t kr = code_row(sq.kc, w.h, key), vr = code_row(sq.vc, w.h, key);
+                if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
+                win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
+                const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key / BLK]);
+                const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key / BLK]);
+                win_e = (ek & 0xffff) | (ev << 16);
+            }
+        };
+        // entry E: K (even) or V (odd) of tile (E - E0) / 2
+        auto load = [&](uint32_t E) {
+            const int i = (int)(E - E0) >> 1, is_v = (int)(E - E0) & 1;
+            if (!is_v && (i & 31) == 0) window(i);
+            const int row = __shfl_sync(0xffffffffu, is_v ? win_v : win_k, i & 31);
+            if (lane == 0) {
+                const uint32_t slot = E % NS;
+                uint8_t *dst = ring + slot * 4096;
+                mbar_expect_tx(&full[slot], 4096);
+                if (is_v) {                          // 32 keys x this warp's 128 dims
+                    tma_load_2d(dst, &p.maps[sq.vmap], 128 * half, row, &full[slot]);
+                    tma_load_2d(dst + 2048, &p.maps[sq.vmap], 128 * half, row + 16, &full[slot]);
+                } else {                             // this warp's 16 keys x 256 dims
+                    tma_load_2d(dst, &p.maps[sq.kmap], 0, row + 16 * half, &full[slot]);
+                    tma_load_2d(dst + 2048, &p.maps[sq.kmap], 128, row + 16 * half, &full[slot]);
+                }
+            }
+        };
+        for (uint32_t E = E0; E < E1 && E < E0 + NS; E++) load(E);
+        for (int row = warp; row < ROWS; row += Cfg::WARPS) stage_q<F32>(p, sq, head0, valid, row, lane, smem + Cfg::OFF_Q, sm_sc + row);
+        if (threadIdx.x < ROWS) sm_lim[threadIdx.x] = (int)threadIdx.x < valid ? sq.base_pos + (int)threadIdx.x / p.gqa : n_keys - 1;
+        __syncthreads();
+
+        float o[NT][8][4];
+        float m[NT][2], l[NT][2], R[NT][2];          // rows 8 n + 2 t and the one after it; R: both halves' maximum
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+            m[n][0] = m[n][1] = R[n][0] = R[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.0f;
+        }
+        const uint32_t q_base = smem_u32(smem + Cfg::OFF_Q) + lane * 16;
+        const uint32_t tok = (uint32_t)(g ^ ((g & 1) << 2));         // this lane group's key of a block of eight
+
+#pragma unroll 1
+        for (int i = 0; i < nt; i++) {
+            const int key0 = (seg_t0 + pair + i * PAIRS) * TILE;
+            const uint32_t EK = E0 + 2 * i, EV = EK + 1;
+            // (the window moves on when the K entry of tile 32 k is asked for, up to two tiles ahead of its use: the
+            // exponents of this tile are read from memory, where the window's lookup has brought them near)
+            const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key0 / BLK]);
+            const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key0 / BLK]);
+
+            // ---- S^T = K Q^T for this warp's 16 keys ----
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            mbar_wait(&full[EK % NS], (EK / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            {
+                const uint32_t kb = smem_u32(ring + (EK % NS) * 4096) + tok * 128;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    uint32_t kw[2][4];                 // keys tok, tok + 8
+#pragma unroll
+                    for (int n = 0; n < 2; n++) lds128(kw[n], kb + (q >> 1) * 2048 + n * 1024 + ((((uint32_t)(4 * (q & 1) + t)) ^ tok) << 4));
+#pragma unroll
+                    for (int kk = 0; kk < 2; kk++) {
+                        uint32_t b[NT][4];             // two k-steps of Q (f32: one, high and low)
+                        if constexpr (!F32) {
+#pragma unroll
+                            for (int n = 0; n < NT; n++) lds128(b[n], q_base + n * 4096 + (q * 2 + kk) * 512);
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int k = kk * 2 + h;
+                            if constexpr (F32) {
+#pragma unroll
+                                for (int n = 0; n < NT; n++) lds128(b[n], q_base + n * 8192 + (q * 4 + k) * 512);
+                            }
+                            const uint32_t a0 = f16x2_lo(kw[0][k]), a1 = f16x2_lo(kw[1][k]), a2 = f16x2_hi(kw[0][k]), a3 = f16x2_hi(kw[1][k]);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                if constexpr (F32) {
+                                    mma_f16(s[n], a0, a1, a2, a3, b[n][0], b[n][1]);
+                                    mma_f16(s[n], a0, a1, a2, a3, b[n][2], b[n][3]);
+                                } else {
+                                    mma_f16(s[n], a0, a1, a2, a3, b[n][2 * h], b[n][2 * h + 1]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (EK + NS < E1) load(EK + NS);
+
+            // ---- weights of the 16 keys against this warp's own maximum, a whole number ----
+            const float fk = pow2f(ek), fv = (float)ev, iv = pow2f(-ev);
+            const bool masked = key0 + TILE > sq.base_pos + 1;
+            uint8_t *px = smem + Cfg::OFF_PX + (pair * 4 + (i & 1) * 2) * Cfg::PX;
+            float *mx = reinterpret_cast<float *>(smem + Cfg::OFF_MX) + (pair * 4 + (i & 1) * 2) * ROWS;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float2 sc = *reinterpret_cast<const float2 *>(sm_sc + n * 8 + 2 * t);
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[n][c] = fmaf(s[n][c], ((c & 1) ? sc.y : sc.x) * fk, fv);
+                if (masked) {
+                    const int2 lim = *reinterpret_cast<const int2 *>(sm_lim + n * 8 + 2 * t);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (key0 + 16 * half + (c >> 1) * 8 + (int)tok > ((c & 1) ? lim.y : lim.x)) s[n][c] = -INFINITY;
+                }
+                float x0 = fmaxf(s[n][0], s[n][2]), x1 = fmaxf(s[n][1], s[n][3]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                }
+                const float n0 = fmaxf(m[n][0], ceilf(x0)), n1 = fmaxf(m[n][1], ceilf(x1));
+                l[n][0] *= m[n][0] == n0 ? 1.0f : ex2(m[n][0] - n0);
+                l[n][1] *= m[n][1] == n1 ? 1.0f : ex2(m[n][1] - n1);
+                m[n][0] = n0; m[n][1] = n1;
+                const float b0 = (n0 == -INFINITY ? 0.0f : n0) - W_SHIFT, b1 = (n1 == -INFINITY ? 0.0f : n1) - W_SHIFT;
+                uint32_t pb[2], pl[2];
+                float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float w0 = ex2(s[n][2 * c] - b0), w1 = ex2(s[n][2 * c + 1] - b1);
+                    a0 += w0; a1 += w1;
+                    const uint32_t hi = pack_f16(w0, w1);
+                    pb[c] = movm(hi);
+                    if constexpr (F32) {
+                        const float2 h = h2f2(hi);
+                        pl[c] = movm(pack_f16(w0 - h.x, w1 - h.y));
+                    }
+                }
+                l[n][0] = fmaf(a0, iv, l[n][0]); l[n][1] = fmaf(a1, iv, l[n][1]);
+                if constexpr (F32) reinterpret_cast<uint4 *>(px + half * Cfg::PX)[n * 32 + lane] = make_uint4(pb[0], pb[1], pl[0], pl[1]);
+                else reinterpret_cast<uint2 *>(px + half * Cfg::PX)[n * 32 + lane] = make_uint2(pb[0], pb[1]);
+                if (g == 0) *reinterpret_cast<float2 *>(mx + half * ROWS + n * 8 + 2 * t) = make_float2(n0, n1);
+            }
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
+
+            // ---- the running output to the common maximum ----
+            bool grow = false;
+            float nr[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float2 a = *reinterpret_cast<const float2 *>(mx + n * 8 + 2 * t), b = *reinterpret_cast<const float2 *>(mx + ROWS + n * 8 + 2 * t);
+                nr[n][0] = fmaxf(a.x, b.x); nr[n][1] = fmaxf(a.y, b.y);
+                grow |= nr[n][0] > R[n][0] || nr[n][1] > R[n][1];
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float f0 = R[n][0] == nr[n][0] ? 1.0f : ex2(R[n][0] - nr[n][0]), f1 = R[n][1] == nr[n][1] ? 1.0f : ex2(R[n][1] - nr[n][1]);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) { o[n][j][0] *= f0; o[n][j][1] *= f1; o[n][j][2] *= f0; o[n][j][3] *= f1; }
+                    R[n][0] = nr[n][0]; R[n][1] = nr[n][1];
+                }
+            }
+
+            // ---- O^T += V^T P^T: row g of tile j is dim 128 half + 16 g + 2 j, row g + 8 the dim after it ----
+            mbar_wait(&full[EV % NS], (EV / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            uint8_t *vs = ring + (EV % NS) * 4096;
+            if (key0 + TILE > n_keys) {                // rows past the last key may hold anything
+                for (int off = (n_keys - key0) * 128 + lane * 16; off < TILE * 128; off += 512) *reinterpret_cast<uint4 *>(vs + off) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+                __syncwarp();
+            }
+            const uint32_t vb = smem_u32(vs);
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {           // the keys of either warp
+                uint32_t b[NT][F32 ? 4 : 2];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    // row g's weights times 2^(own maximum - common maximum), in two steps (fp16 ends at 2^-24)
+                    const float ma = mx[kk * ROWS + n * 8 + g], mb = mx[(kk ^ 1) * ROWS + n * 8 + g];
+                    const float d = ma >= mb ? 0.0f : fmaxf(ma - mb, -40.0f);
+                    const float d0 = fmaxf(d, -14.0f), d1 = fmaxf(d - d0, -24.0f);
+                    const __half2 f0 = __float2half2_rn(ex2(d0)), f1 = __float2half2_rn(ex2(d1));
+                    if constexpr (F32) {
+                        const uint4 v = reinterpret_cast<const uint4 *>(px + kk * Cfg::PX)[n * 32 + lane];
+                        b[n][0] = v.x; b[n][1] = v.y; b[n][2] = v.z; b[n][3] = v.w;
+                    } else {
+                        const uint2 v = reinterpret_cast<const uint2 *>(px + kk * Cfg::PX)[n * 32 + lane];
+                        b[n][0] = v.x; b[n][1] = v.y;
+                    }
+#pragma unroll
+                    for (int c = 0; c < (F32 ? 4 : 2); c++) {
+                        const __half2 x = __hmul2(__hmul2(*reinterpret_cast<const __half2 *>(&b[n][c]), f0), f1);
+                        b[n][c] = *reinterpret_cast<const uint32_t *>(&x);
+                    }
+                }
+                const uint32_t ta = 16 * kk + 2 * t, tb = 16 * kk + ((2 * t + 1) ^ 4);
+                uint32_t v[4][4];                      // keys ta, tb, ta + 8, tb + 8
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t tk = ((c & 1) ? tb : ta) + (c >> 1) * 8;
+                    lds128(v[c], vb + tk * 128 + (((uint32_t)g ^ (tk & 7)) << 4));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t p0 = __byte_perm(v[0][k], v[1][k], 0x5140), p1 = __byte_perm(v[0][k], v[1][k], 0x7362);
+                    const uint32_t r0 = __byte_perm(v[2][k], v[3][k], 0x5140), r1 = __byte_perm(v[2][k], v[3][k], 0x7362);
+                    const uint32_t c0 = f16x2_lo(p0), c1 = f16x2_hi(p0), c2 = f16x2_lo(r0), c3 = f16x2_hi(r0);
+                    const uint32_t d0 = f16x2_lo(p1), d1 = f16x2_hi(p1), d2 = f16x2_lo(r1), d3 = f16x2_hi(r1);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma_f16(o[n][2 * k], c0, c1, c2, c3, b[n][0], b[n][1]);
+                        mma_f16(o[n][2 * k + 1], d0, d1, d2, d3, b[n][0], b[n][1]);
+                        if constexpr (F32) {
+                            mma_f16(o[n][2 * k], c0, c1, c2, c3, b[n][2], b[n][3]);
+                            mma_f16(o[n][2 * k + 1], d0, d1, d2, d3, b[n][2], b[n][3]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (EV + NS < E1) load(EV + NS);
+        }
+        E0 = E1;
+
+        // ---- segment end: every warp puts its 128 dims of all rows into its slots, and all threads add them up ----
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], d);
+                if (g == 0) { sm_m[warp * ROWS + n * 8 + 2 * t + c] = m[n][c]; sm_l[warp * ROWS + n * 8 + 2 * t + c] = l[n][c]; }
+            }
+        }
+        if (nt > 0) {
+            // piece c (four dims) of a row sits at c ^ ((row >> 1) & 3), which spreads a phase's eight lanes over the banks
+            float *own = reinterpret_cast<float *>(ring);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t piece = (uint32_t)(g * 4 + e) ^ (uint32_t)t;
+                    const int row = n * 8 + 2 * t;
+                    *reinterpret_cast<float4 *>(own + row * 128 + piece * 4) = make_float4(o[n][2 * e][0], o[n][2 * e][2], o[n][2 * e + 1][0], o[n][2 * e + 1][2]);
+                    *reinterpret_cast<float4 *>(own + (row + 1) * 128 + piece * 4) = make_float4(o[n][2 * e][1], o[n][2 * e][3], o[n][2 * e + 1][1], o[n][2 * e + 1][3]);
+                }
+        }
+        __syncthreads();
+        const bool whole = seg_t0 == 0 && seg_n == sq.n_tiles;
+        const size_t slot = (size_t)blockIdx.x + (size_t)w.s * p.kv_heads + w.h;
+        const int in = min(PAIRS, seg_n);              // pairs that had a tile
+        for (int idx = threadIdx.x; idx < valid * 64; idx += Cfg::THREADS) {
+            const int row = idx >> 6, pc = idx & 63;
+            const uint32_t piece = (uint32_t)(pc & 31) ^ (uint32_t)((row >> 1) & 3);
+            float M = -INFINITY;
+            for (int k = 0; k < 2 * in; k++) M = fmaxf(M, sm_m[k * ROWS + row]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.0f;
+            for (int k = 0; k < in; k++) {
+                const float ma = sm_m[2 * k * ROWS + row], mb = sm_m[(2 * k + 1) * ROWS + row], r = fmaxf(ma, mb);
+                const float f = r == M ? 1.0f : ex2(r - M);
+                L += sm_l[2 * k * ROWS + row] * (ma == M ? 1.0f : ex2(ma - M)) + sm_l[(2 * k + 1) * ROWS + row] * (mb == M ? 1.0f : ex2(mb - M));
+                const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + (2 * k + (pc >> 5)) * NS * 4096) + row * 128 + piece * 4);
+                acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y); acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+            }
+            if (whole) {
+                const int r = row / p.gqa;
+                const float inv = 1.0f / L;
+                store_out(p, sq, (size_t)r * p.q_heads + head0 + (row - r * p.gqa), pc * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+            } else {
+                const size_t pi = slot * p.slot_rows + row;
+                *reinterpret_cast<float4 *>(p.pacc + pi * 256 + pc * 4) = acc;
+                if (pc == 0) *reinterpret_cast<float2 *>(p.pstat + pi * 2) = make_float2(M, L);
+            }
+        }
+        T += seg_n;
+        w.t = 0;                                          // the next segment, if any, begins the next group
+        if (++w.h == p.kv_heads) { w.h = 0; w.s++; }
+        fence_proxy_async();                              // the ring goes back to the copy engine
+        __syncthreads();
+    }
+    if (*abort_flag)                                      // a wait gave up: copies of this CTA may still be under way
+        for (int i = 0; i < 4096; i++) __nanosleep(10000);
+}
+
 // Partials of a cut group: one block per (group, row).  Slices of 64 threads x four dims take every MG_SLICES-th
 // partial each, ten loads in flight, asked for before the weights are known: one trip to L2 for up to 40 partials
 // (four slices: many groups, few partials each) or 160 (sixteen: few groups, cut over most of the SMs).
@@ -1078,22 +1070,6 @@ void pdl_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &attr, dim3 grid, u
     cfg.attrs = &attr; cfg.numAttrs = g_tune_pdl ? 1 : 0;
 }
 
-template <int MT, bool F32>
-void launch_attn_t(cudaStream_t s, const Kv8AttnParams &p) {
-    static bool configured[64] = {false};      // the attribute is per device
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && !configured[dev]) {
-        cudaFuncSetAttribute(kv8_attn_kernel<MT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, AtCfg<MT>::SMEM);
-        configured[dev] = true;
-    }
-    cudaLaunchConfig_t cfg;
-    cudaLaunchAttribute attr;
-    pdl_config(cfg, attr, dim3((unsigned)p.n_cta), AT_THREADS, AtCfg<MT>::SMEM, s);
-    cudaLaunchKernelEx(&cfg, kv8_attn_kernel<MT, F32>, p);
-    g_launches++;
-}
-
 template <bool F32>
 void launch_decode_t(cudaStream_t s, const Kv8AttnParams &p) {
     static bool configured[64] = {false};      // the attribute is per device
@@ -1107,6 +1083,23 @@ void launch_decode_t(cudaStream_t s, const Kv8AttnParams &p) {
     cudaLaunchAttribute attr;
     pdl_config(cfg, attr, dim3((unsigned)p.n_cta), D_THREADS, D_SMEM, s);
     cudaLaunchKernelEx(&cfg, kv8_decode_kernel<F32>, p);
+    g_launches++;
+}
+
+template <int NT, bool F32>
+void launch_verify_t(cudaStream_t s, const Kv8AttnParams &p) {
+    using Cfg = VfCfg<NT, F32>;
+    static bool configured[64] = {false};      // the attribute is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !configured[dev]) {
+        cudaFuncSetAttribute(kv8_verify_kernel<NT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+        configured[dev] = true;
+    }
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(cfg, attr, dim3((unsigned)p.n_cta), Cfg::THREADS, Cfg::SMEM, s);
+    cudaLaunchKernelEx(&cfg, kv8_verify_kernel<NT, F32>, p);
     g_launches++;
 }
 
@@ -1171,12 +1164,12 @@ void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scrat
     const size_t slots = (size_t)p.n_cta + (size_t)p.n_seq * p.kv_heads;
     p.pacc = reinterpret_cast<float *>(scratch);
     p.pstat = p.pacc + slots * p.slot_rows * 256;
-    const int valid = max_rows * p.gqa, f32 = p.io == DT_F32, per = f32 ? 8 : 16;
-    const int mt = (valid + per - 1) / per;
-    if (valid <= 8) { if (f32) launch_decode_t<true>(s, p); else launch_decode_t<false>(s, p); }
-    else
-    if (f32) { if (mt <= 1) launch_attn_t<1, true>(s, p); else if (mt <= 2) launch_attn_t<2, true>(s, p); else launch_attn_t<4, true>(s, p); }
-    else { if (mt <= 1) launch_attn_t<1, false>(s, p); else if (mt <= 2) launch_attn_t<2, false>(s, p); else launch_attn_t<4, false>(s, p); }
+    const int valid = max_rows * p.gqa, nt = (valid + 7) / 8;
+    const bool f32 = p.io == DT_F32;
+    if (nt <= 1) { if (f32) launch_decode_t<true>(s, p); else launch_decode_t<false>(s, p); }
+    else if (nt == 2) { if (f32) launch_verify_t<2, true>(s, p); else launch_verify_t<2, false>(s, p); }
+    else if (nt == 3) { if (f32) launch_verify_t<3, true>(s, p); else launch_verify_t<3, false>(s, p); }
+    else { if (f32) launch_verify_t<4, true>(s, p); else launch_verify_t<4, false>(s, p); }
     int parts = 0;                             // most partials of a cut group
     for (int i = 0; i < p.n_seq; i++)
         for (int h = 0; h < p.kv_heads; h++) {

@@ -210,7 +210,7 @@ struct Pool {
     int refs;                             // arenas (and the pool's own handle) that keep it alive
     CUtensorMap map;                      // 32-row boxes (split-KV kernel)
     CUtensorMap map64;                    // 64-row boxes (prefill kernel)
-    CUtensorMap map8;                     // the same range as 256-byte rows of 8-bit codes, boxes of 128 bytes x 32 rows
+    CUtensorMap map8[3];                  // the same range as 256-byte rows of 8-bit codes, boxes of 128 bytes x 16, 32, 64 rows
 };
 struct Arena {
     Pool *pool;
@@ -237,13 +237,25 @@ bool encode_rows_map(CUtensorMap *m, void *base, uint64_t rows, uint32_t box_row
     return true;
 }
 
-// Rows of 256 one-byte codes, as boxes of 128 codes x 32 rows.
-bool encode_codes_map(CUtensorMap *m, void *base, uint64_t rows) {
+// Rows of 256 one-byte codes, as boxes of 128 codes x box_rows.
+bool encode_codes_map(CUtensorMap *m, void *base, uint64_t rows, uint32_t box_rows) {
     cuuint64_t dims[2] = {QW_HEAD_DIM, rows};
     cuuint64_t strides[1] = {QW_HEAD_DIM};
-    cuuint32_t box[2] = {128, 32};
+    cuuint32_t box[2] = {128, box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = G.encodeTiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed (%d)", (int)r); return false; }
+    return true;
+}
+
+// [rows][heads][256] bf16, heads head_pitch elements apart, as boxes of 64 dims x box_heads x box_rows.
+bool encode_heads_map(CUtensorMap *m, const void *base, uint64_t rows, uint64_t heads, uint64_t head_pitch, uint32_t box_heads, uint32_t box_rows) {
+    cuuint64_t dims[3] = {QW_HEAD_DIM, heads, rows};
+    cuuint64_t strides[2] = {head_pitch * 2, heads * head_pitch * 2};
+    cuuint32_t box[3] = {64, box_heads, box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = G.encodeTiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed (%d)", (int)r); return false; }
     return true;
@@ -404,7 +416,9 @@ Pool *pool_create(size_t max_bytes, uint32_t shuffle) {
     // the tensor maps span the whole reserved range; rows of unmapped pages are never addressed
     if (!encode_rows_map(&pl->map, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 512), 32) ||
         !encode_rows_map(&pl->map64, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 512), 64) ||
-        !encode_codes_map(&pl->map8, reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 256))) { pool_release(pl); return nullptr; }
+        !encode_codes_map(&pl->map8[0], reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 256), 16) ||
+        !encode_codes_map(&pl->map8[1], reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 256), 32) ||
+        !encode_codes_map(&pl->map8[2], reinterpret_cast<void *>(pl->va), (uint64_t)(pl->va_size / 256), 64)) { pool_release(pl); return nullptr; }
     return pl;
 }
 
@@ -571,7 +585,7 @@ size_t kv8_layer_bytes(int32_t kv_heads, int32_t max_ctx) {
 
 // One layer of an 8-bit cache -> Kv8Layer + tensor map; `append`: the pages of [first_token, n_tokens) are mapped.
 bool resolve_kv8(qw_cmd c, qw_ref ref, int32_t kv_heads, int32_t max_ctx, int32_t first_token, int32_t n_tokens, bool append,
-                 Kv8Layer *out, CUtensorMap *map) {
+                 Kv8Layer *out, CUtensorMap *map, uint32_t box_rows = 32) {
     qw_buf b = ref.buf;
     if (!b) { cmd_fail(c, "cache operand is null"); return false; }
     if (b->kind == BUF_POOL) { cmd_fail(c, "a page pool is not a cache: allocate an arena in it"); return false; }
@@ -600,7 +614,7 @@ bool resolve_kv8(qw_cmd c, qw_ref ref, int32_t kv_heads, int32_t max_ctx, int32_
         out->table = a->table_dev + (size_t)layer * kv_heads * a->pages_per_head;
         out->pt_stride = a->pages_per_head;
         out->exps = a->exps_dev + (size_t)layer * kv_heads * out->exp_stride;
-        if (map) *map = a->pool->map8;
+        if (map) *map = a->pool->map8[box_rows == 16 ? 0 : box_rows == 32 ? 1 : 2];
         return true;
     }
     uint8_t *d = (uint8_t *)dev_range(c, ref, layer_bytes, append, 128);
@@ -611,11 +625,11 @@ bool resolve_kv8(qw_cmd c, qw_ref ref, int32_t kv_heads, int32_t max_ctx, int32_
     out->exps = d + (size_t)kv_heads * max_ctx * QW_HEAD_DIM;
     if (map) {
         const uint64_t rows = (uint64_t)kv_heads * max_ctx;
-        const auto key = std::make_pair((uintptr_t)d, rows | (uint64_t)1 << 63);      // (bf16 maps: rows * 128 + box rows)
+        const auto key = std::make_pair((uintptr_t)d, rows * 128 + box_rows | (uint64_t)1 << 63);      // (bf16 maps: without the top bit)
         auto it = G.map_cache.find(key);
         if (it == G.map_cache.end()) {
             CUtensorMap m;
-            if (!encode_codes_map(&m, d, rows)) { cmd_fail(c, "%s", SH.last_error); return false; }
+            if (!encode_codes_map(&m, d, rows, box_rows)) { cmd_fail(c, "%s", SH.last_error); return false; }
             it = G.map_cache.emplace(key, m).first;
         }
         *map = it->second;
@@ -724,9 +738,6 @@ struct SplitBatch {
 // With cs_table != nullptr, q_bf16 is instead the raw [rows, q_heads, 512] bf16 [q|gate] input: the kernel
 // norms (weights q_norm_w or nullptr, eps) and rotates its own query tiles, with the angles' cos / sin from
 // cs_table ([rows, 64] f32, left by the pre-op).
-bool run_prefill_on(qw_cmd c, PrefillParams &p, int64_t k_rows, int64_t v_rows, const __nv_bfloat16 *q_bf16, void *out, int out_dtype,
-                    const void *gate, int gate_dtype, int gate_stride, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t base_pos,
-                    float scale, const float *cs_table = nullptr, const uint16_t *q_norm_w = nullptr, float eps = 0.0f);
 bool run_prefill(qw_cmd c, const __nv_bfloat16 *q_bf16, void *out, int out_dtype, const void *gate, int gate_dtype,
                  int gate_stride, qw_ref kcache, qw_ref vcache, int32_t rows, int32_t q_heads, int32_t kv_heads,
                  int32_t max_ctx, int32_t base_pos, float scale, const float *cs_table = nullptr,
@@ -736,13 +747,6 @@ bool run_prefill(qw_cmd c, const __nv_bfloat16 *q_bf16, void *out, int out_dtype
     int64_t k_rows = 0, v_rows = 0;
     if (!resolve_cache(c, kcache, kv_heads, max_ctx, QW_HEAD_DIM, base_pos + rows, false, false, &p.kc, &p.kmap, 64, &k_rows)) return false;
     if (!resolve_cache(c, vcache, kv_heads, max_ctx, QW_HEAD_DIM, base_pos + rows, false, false, &p.vc, &p.vmap, 64, &v_rows)) return false;
-    return run_prefill_on(c, p, k_rows, v_rows, q_bf16, out, out_dtype, gate, gate_dtype, gate_stride, rows, q_heads, kv_heads, base_pos,
-                          scale, cs_table, q_norm_w, eps);
-}
-
-bool run_prefill_on(qw_cmd c, PrefillParams &p, int64_t k_rows, int64_t v_rows, const __nv_bfloat16 *q_bf16, void *out, int out_dtype,
-                    const void *gate, int gate_dtype, int gate_stride, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t base_pos,
-                    float scale, const float *cs_table, const uint16_t *q_norm_w, float eps) {
     p.q = q_bf16;
     p.out = out; p.out_dtype = out_dtype; p.gate = gate; p.gate_dtype = gate_dtype; p.gate_stride = gate_stride;
     p.rows = rows; p.base_pos = base_pos; p.q_heads = q_heads; p.kv_heads = kv_heads; p.gqa = q_heads / kv_heads;
@@ -2110,31 +2114,37 @@ struct Kv8Call {
     int32_t base_pos;
 };
 
-// Many bf16 rows: the cache is widened to bf16 once (a code times a power of two is a bf16 number) and the tcgen05
-// prefill kernel runs over the copy.
-bool kv8_prefill(qw_cmd c, const Kv8Layer &kc, const Kv8Layer &vc, const void *q, void *out, const void *gate, int32_t rows, int32_t q_heads,
-                 int32_t kv_heads, int32_t base_pos, float scale, int32_t gate_stride) {
-    const int n = base_pos + rows;
-    const size_t one = (size_t)kv_heads * n * QW_HEAD_DIM * 2;
-    char *scr = (char *)cmd_scratch(c, 2 * one);
-    if (!scr) return false;
-    launch_kv8_read(c->stream, scr, DT_BF16, kc, kv_heads, 0, n);
-    launch_kv8_read(c->stream, scr + one, DT_BF16, vc, kv_heads, 0, n);
-    PrefillParams p;
+// Many bf16 rows: the tcgen05 kernel.
+bool kv8_prefill(qw_cmd c, const Kv8Call &a, const void *q, void *out, const void *gate, int32_t rows, int32_t q_heads, int32_t kv_heads,
+                 int32_t max_ctx, float scale, int32_t gate_stride) {
+    Kv8PrefillParams p;
     memset(&p, 0, sizeof p);
-    const int64_t map_rows = (int64_t)kv_heads * n;
-    if (!encode_rows_map(&p.kmap, scr, map_rows, 64) || !encode_rows_map(&p.vmap, scr + one, map_rows, 64))
+    const int32_t end = a.base_pos + rows;
+    if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &p.kc, &p.kmap, 64) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &p.vc, &p.vmap, 64)) return false;
+    p.gqa = q_heads / kv_heads;
+    p.tile_rows = 128 / p.gqa;
+    if (!encode_heads_map(&p.qmap, q, rows, q_heads, QW_HEAD_DIM, p.gqa, p.tile_rows) || !encode_heads_map(&p.omap, out, rows, q_heads, QW_HEAD_DIM, p.gqa, p.tile_rows) ||
+        (gate && !encode_heads_map(&p.gmap, gate, rows, q_heads, gate_stride, p.gqa, p.tile_rows)))
         return cmd_fail(c, "%s", SH.last_error), false;
-    p.kc.base = reinterpret_cast<__nv_bfloat16 *>(scr); p.kc.max_ctx = n;
-    p.vc.base = reinterpret_cast<__nv_bfloat16 *>(scr + one); p.vc.max_ctx = n;
-    return run_prefill_on(c, p, map_rows, map_rows, reinterpret_cast<const __nv_bfloat16 *>(q), out, DT_BF16, gate, DT_BF16, gate_stride, rows,
-                          q_heads, kv_heads, base_pos, scale);
+    p.out = reinterpret_cast<__nv_bfloat16 *>(out);
+    p.gate = reinterpret_cast<const __nv_bfloat16 *>(gate);
+    p.gate_stride = gate_stride; p.gated = gate != nullptr;
+    p.rows = rows; p.base_pos = a.base_pos; p.q_heads = q_heads; p.kv_heads = kv_heads;
+    p.n_q_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+    p.box_bytes = 128 * p.gqa * p.tile_rows;
+    p.splits = kv8_prefill_splits(p.n_q_tiles * kv_heads, (a.base_pos + (rows + 1) / 2 + 127) / 128, sm_count());
+    p.scale = scale;
+    p.status = cmd_status(c);
+    void *scr = nullptr;
+    if (p.splits > 1 && !(scr = cmd_scratch(c, kv8_prefill_scratch_bytes(p)))) return false;
+    launch_kv8_prefill(c->stream, p, scr);
+    return cuda_ok(c, cudaGetLastError(), "attn_kv8 launch");
 }
 
 bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_ctx,
               float scale, int32_t gate_stride, qw_dtype io) {
     if (!kv8_shape(c, "attn_kv8", kv_heads, head_dim, max_ctx, io)) return false;
-    const int most = kv8_max_query_rows(io), gqa = q_heads > 0 ? q_heads / kv_heads : 0;
+    const int most = KV8_MAX_QUERY_ROWS, gqa = q_heads > 0 ? q_heads / kv_heads : 0;
     if (q_heads <= 0 || q_heads % kv_heads || gqa > most) { cmd_fail(c, "attn_kv8: %d query heads over %d (at most %d to one) not supported", q_heads, kv_heads, most); return false; }
     const size_t el = io == QW_BF16 ? 2 : 4;
     for (int i = 0; i < n_seq; i++) {
@@ -2149,6 +2159,9 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
     if (rows == 0) return true;
     const size_t n = (size_t)rows * q_heads, bytes = n * QW_HEAD_DIM * el;
     const int chunk = std::max(1, most / gqa);
+    const uint32_t box = kv8_box_rows(std::min(rows, chunk) * gqa);
+    // many bf16 rows on the tcgen05 kernel (which needs a scale it can multiply masked scores by)
+    const bool tiled = rows * gqa > most && io == QW_BF16 && fabsf(scale) > 1e-12f && fabsf(scale) < 1e12f;
     Kv8AttnParams p;
     memset(&p, 0, sizeof p);
     p.q_heads = q_heads; p.kv_heads = kv_heads; p.gqa = gqa; p.io = io; p.gate_stride = gate_stride; p.scale = scale;
@@ -2167,7 +2180,7 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
     auto map_slot = [&](const CUtensorMap &m) {
         for (int i = 0; i < n_maps; i++)
             if (!memcmp(&p.maps[i], &m, sizeof m)) return i;
-        if (n_maps == QW_MAX_MAPS) return -1;
+        if (n_maps == QW_KV8_MAPS) return -1;
         p.maps[n_maps] = m;
         return n_maps++;
     };
@@ -2176,14 +2189,14 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
         Kv8Layer kc, vc;
         CUtensorMap km, vm;
         const int32_t end = a.base_pos + rows;
-        if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &kc, &km) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &vc, &vm)) return false;
+        if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &kc, &km, box) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &vc, &vm, box)) return false;
         const char *qp = (const char *)near_range(c, a.q, bytes, false);
         char *op = (char *)near_range(c, a.out, bytes, true);
         const char *gp = a.gate.buf ? (const char *)near_range(c, a.gate, ((n - 1) * gate_stride + QW_HEAD_DIM) * el, false) : nullptr;
         if (!qp || !op || (a.gate.buf && !gp)) return false;
-        if (rows * gqa > most && io == QW_BF16 && attn_prefill_io_ok(op, DT_BF16, gp, DT_BF16, gate_stride)) {
+        if (tiled && attn_prefill_io_ok(op, DT_BF16, gp, DT_BF16, gate_stride)) {
             if (!flush()) return false;
-            if (!kv8_prefill(c, kc, vc, qp, op, gp, rows, q_heads, kv_heads, a.base_pos, scale, gate_stride)) return false;
+            if (!kv8_prefill(c, a, qp, op, gp, rows, q_heads, kv_heads, max_ctx, scale, gate_stride)) return false;
             continue;
         }
         for (int r0 = 0; r0 < rows; r0 += chunk) {
