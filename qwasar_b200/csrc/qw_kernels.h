@@ -285,7 +285,7 @@ void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scrat
 
 // Many bf16 rows over an 8-bit cache on tcgen05 (qw_kv8_prefill.cu).
 struct Kv8PrefillParams {
-    CUtensorMap kmap, vmap;  // code rows, boxes of 128 bytes x 64 rows
+    CUtensorMap kmap;        // K code rows, boxes of 128 bytes x 64 rows
     // [rows][q_heads][256] bf16 tensors (gate: heads gate_stride apart), boxes of 64 dims x gqa heads x tile_rows rows
     CUtensorMap qmap, omap, gmap;
     Kv8Layer kc, vc;

@@ -4,9 +4,9 @@
 // with all query heads of the kv head: tile row i is row i / grouping, head i % grouping, so K and V are read once for
 // the whole group.  128 keys per step:
 //
-//   warp 9       TMA: K codes (two stages of 128 keys x 256 dims, 32 KB)
-//   warp 10      TMA: the Q tile, then V codes (two stages of 64 keys x 256 dims, 16 KB)
-//   warps 12-15  widen V codes to fp16 (exact) into two 32 KB stages, keys past the last one as zeros
+//   warp 9       TMA: the Q tile, then K codes (two stages of 128 keys x 256 dims, 32 KB)
+//   warps 12-15  V: codes from memory into registers, 64 keys ahead, widened to fp16 (exact) into three 32 KB stages of
+//                64 keys; keys past the last one are zeros
 //   warp 8       one thread issues  S  = Q K_j^T   (kind::f8f6f4: the K codes enter as they lie in the cache)
 //   warp 11      one thread issues  O += P_j V_j   (kind::f16, P in tensor memory)
 //   warps 0-7    softmax: two threads per tile row, 64 keys of every step each -- one block of the cache, so one
@@ -34,25 +34,25 @@ namespace {
 
 constexpr int BM = 128, BN = 128;
 constexpr int K_BYTES = BN * 256, KBOX = BN * 128;    // K stage; 128 dims of it
-constexpr int V8_BYTES = 64 * 256, V8BOX = 64 * 128;  // V codes of 64 keys; 128 dims of them
 constexpr int V_BYTES = 64 * 512, VBOX = 64 * 128;    // V fp16 of 64 keys; 64 dims of them
+constexpr int V_ST = 3;
 constexpr int IO_BOX = BM * 128;
-constexpr int OFF_K = 0, OFF_V = 2 * K_BYTES, OFF_V8 = OFF_V + 2 * V_BYTES, OFF_QLO = OFF_V8 + 2 * V8_BYTES;
+constexpr int OFF_K = 0, OFF_V = 2 * K_BYTES, OFF_QLO = OFF_V + V_ST * V_BYTES;
 constexpr int OFF_BAR = OFF_QLO + 2 * IO_BOX;
 constexpr int OFF_STAGE_Q = OFF_V, OFF_STAGE_IO = OFF_K;      // Q tile (4 boxes bf16); gate / output (4 boxes), partial sums (8 boxes)
-static_assert(OFF_V == 4 * IO_BOX && 2 * V_BYTES == 4 * IO_BOX, "a share's sums take the K and the V stages");
+static_assert(OFF_V == 4 * IO_BOX && V_ST * V_BYTES >= 4 * IO_BOX, "a share's sums take the K and the V stages");
 constexpr int COL_O = 0, COL_Q = 256, COL_P = 320, COL_S = 384;
 constexpr int OFF_XCH = OFF_BAR + 256;                        // row maxima / sums passed between the two softmax halves
 constexpr int SMEM_BYTES = OFF_XCH + 2 * 2 * BM * 4;
 static_assert(SMEM_BYTES <= 232448, "exceeds the 227 KB a CTA may use");
 constexpr int THREADS = 16 * 32;
-constexpr int W_MMA = 8, W_K = 9, W_V = 10, W_PV = 11, W_CV = 12;
+constexpr int W_MMA = 8, W_K = 9, W_PV = 11, W_CV = 12;       // (warp 10: none)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG_BIG = -1.0e30f;
 constexpr float RESCALE_AT = 8.0f, P_SHIFT = 7.0f;
 
-enum Bar { Q_READY = 0, Q_FULL, G_FULL, K_FULL0, K_FULL1, K_FREE0, K_FREE1, V8_FULL0, V8_FULL1, V8_FREE0, V8_FREE1,
-           V_FULL0, V_FULL1, V_FREE0, V_FREE1, S_READY, S_FREE, P_READY, PV_DONE, PV_ISSUED, N_BARS };
+enum Bar { Q_READY = 0, Q_FULL, G_FULL, K_FULL0, K_FULL1, K_FREE0, K_FREE1, V_FULL0, V_FULL1, V_FULL2, V_FREE0, V_FREE1, V_FREE2,
+           S_READY, S_FREE, P_READY, PV_DONE, PV_ISSUED, N_BARS };
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < N_BARS; i++)
-            mbar_init(&bars[i], (i == P_READY || i == S_FREE || i == Q_READY) ? 8 : (i == V8_FREE0 || i == V8_FREE1 || i == V_FULL0 || i == V_FULL1) ? 4 : 1);
+            mbar_init(&bars[i], (i == P_READY || i == S_FREE || i == Q_READY) ? 8 : (i >= V_FULL0 && i <= V_FULL2) ? 4 : 1);
         *abort_flag = 0;
         mbar_fence_init();
     }
@@ -209,6 +209,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
 
     if (warp == W_K) {
         if (lane == 0) {
+            mbar_expect_tx(&bars[Q_FULL], 4 * p.box_bytes);
+            for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_Q + b * IO_BOX, &p.qmap, b * 64, kvh * p.gqa, r0, &bars[Q_FULL]);
             for (int j = 0; j < n_t; j++) {
                 const int st = j & 1;
                 const int32_t r = step_row(p.kc, j);
@@ -226,19 +228,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
                 mbar_wait(&bars[K_FREE0 + ((n_t - 1) & 1)], ((n_t - 1) >> 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
                 mbar_expect_tx(&bars[G_FULL], 4 * p.box_bytes);
                 for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_IO + b * IO_BOX, &p.gmap, b * 64, kvh * p.gqa, r0, &bars[G_FULL]);
-            }
-        }
-    } else if (warp == W_V) {
-        if (lane == 0) {
-            mbar_expect_tx(&bars[Q_FULL], 4 * p.box_bytes);
-            for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_Q + b * IO_BOX, &p.qmap, b * 64, kvh * p.gqa, r0, &bars[Q_FULL]);
-            for (int pg = 0; pg < 2 * n_t; pg++) {
-                const int st = pg & 1;
-                const int32_t r = step_row(p.vc, pg >> 1) + (pg & 1) * 64;
-                if (pg >= 2) mbar_wait(&bars[V8_FREE0 + st], ((pg >> 1) - 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
-                mbar_expect_tx(&bars[V8_FULL0 + st], V8_BYTES);
-                tma_load_2d(smem + OFF_V8 + st * V8_BYTES, &p.vmap, 0, r, &bars[V8_FULL0 + st]);
-                tma_load_2d(smem + OFF_V8 + st * V8_BYTES + V8BOX, &p.vmap, 128, r, &bars[V8_FULL0 + st]);
             }
         }
     } else if (warp == W_MMA) {
@@ -276,21 +265,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
             constexpr uint32_t idesc_pv = instr_desc(128, 256, 1);
             constexpr uint32_t hi = desc_hi(1024);
             const uint32_t v_a = smem_u32(smem + OFF_V);
+            int st = 0;
+            uint32_t ph = 0;                                 // stage and parity of the next 64 keys
             for (int j = 0; j < n_t; j++) {
-                mbar_wait_hot(&bars[V_FULL0], j & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+                mbar_wait_hot(&bars[V_FULL0 + st], ph, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
                 mbar_wait_hot(&bars[P_READY], j & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
                 tc_fence_after();
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if (h == 1) {
-                        mbar_wait_hot(&bars[V_FULL1], j & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+                        mbar_wait_hot(&bars[V_FULL0 + st], ph, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
                         tc_fence_after();
                     }
-                    const uint32_t v_lo = desc_lo(v_a + h * V_BYTES, VBOX);
+                    const uint32_t v_lo = desc_lo(v_a + st * V_BYTES, VBOX);
 #pragma unroll
                     for (int ks = 0; ks < 4; ks++)       // 16 keys: 8 columns of P, 2048 bytes of V
                         mma_ts_f16(j > 0 || h > 0 || ks > 0, t_o, t_p + (h * 4 + ks) * 8, v_lo + ks * 128, hi, idesc_pv);
-                    tc_commit(&bars[V_FREE0 + h]);
+                    tc_commit(&bars[V_FREE0 + st]);
+                    if (++st == V_ST) { st = 0; ph ^= 1; }
                 }
                 tc_commit(&bars[PV_DONE]);
                 mbar_arrive(&bars[PV_ISSUED]);
@@ -298,22 +290,31 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
         }
     } else if (warp >= W_CV) {
         // ---------------- V codes -> fp16 ----------------
-        // Eight lanes take the eight 16-byte pieces (16 dims) of a 128-byte code row, which become two 16-byte pieces of
-        // the fp16 row each; lanes 4-7 of the eight write their second piece first, so that a store meets all banks.
-        const int u0 = (warp - W_CV) * 32 + lane, c = u0 & 7;
-        mbar_wait(&bars[Q_READY], 0, abort_flag, p.status, QW_ST_MMA_TIMEOUT);     // the Q tile was staged here
-        for (int pg = 0; pg < 2 * n_t; pg++) {
-            const int st = pg & 1;
-            if (pg >= 2) mbar_wait(&bars[V_FREE0 + st], ((pg >> 1) - 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
-            mbar_wait(&bars[V8_FULL0 + st], (pg >> 1) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-            const int left = n_keys - (j0 * BN + pg * 64);         // keys from here on are past the last one: zeros
+        // Eight lanes take the eight 16-byte pieces (16 dims) of half a code row, which become two 16-byte pieces of the
+        // fp16 row each; lanes 4-7 of the eight write their second piece first, so that a store meets all banks.  The
+        // codes of the 64 keys after the next are on their way while a stage is filled.
+        const int u0 = (warp - W_CV) * 32 + lane, c = u0 & 7, k0 = u0 >> 3;
+        const int n_pg = 2 * n_t;
+        auto fetch = [&](uint4(&q)[8], int pg) {
+            if (pg >= n_pg) return;
+            const uint8_t *src = p.vc.base + ((int64_t)step_row(p.vc, pg >> 1) + (pg & 1) * 64 + k0) * 256 + c * 16;
+            const int left = n_keys - (j0 * BN + pg * 64) - k0;    // keys from here on are past the last one
+#pragma unroll
+            for (int i = 0; i < 8; i++) {                          // half i & 1 of key k0 + 16 (i / 2)
+                q[i] = make_uint4(0, 0, 0, 0);
+                if (16 * (i >> 1) < left) q[i] = __ldcg(reinterpret_cast<const uint4 *>(src + (i >> 1) * 4096 + (i & 1) * 128));
+            }
+        };
+        int st = 0;
+        uint32_t ph = 1;                                           // parity of the stage's last release (first round: none)
+        auto put = [&](const uint4(&q)[8], int pg) {
+            if (pg >= n_pg) return;
+            if (pg >= V_ST) mbar_wait(&bars[V_FREE0 + st], ph, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const int x = i & 1, key = (u0 >> 3) + 16 * (i >> 1);
-                uint4 q = *reinterpret_cast<const uint4 *>(smem + OFF_V8 + st * V8_BYTES + x * V8BOX + key * 128 + ((c ^ (key & 7)) << 4));
-                if (key >= left) q = make_uint4(0, 0, 0, 0);
-                const uint4 a = make_uint4(f16x2_of(q.x), f16x2_of(q.x >> 16), f16x2_of(q.y), f16x2_of(q.y >> 16));
-                const uint4 b = make_uint4(f16x2_of(q.z), f16x2_of(q.z >> 16), f16x2_of(q.w), f16x2_of(q.w >> 16));
+                const int x = i & 1, key = k0 + 16 * (i >> 1);
+                const uint4 a = make_uint4(f16x2_of(q[i].x), f16x2_of(q[i].x >> 16), f16x2_of(q[i].y), f16x2_of(q[i].y >> 16));
+                const uint4 b = make_uint4(f16x2_of(q[i].z), f16x2_of(q[i].z >> 16), f16x2_of(q[i].w), f16x2_of(q[i].w >> 16));
                 uint8_t *box = smem + OFF_V + st * V_BYTES + (x * 2 + (c >> 2)) * VBOX + key * 128;
                 const uint32_t d0 = (uint32_t)(((c & 3) * 2) ^ (key & 7)) << 4, d1 = d0 ^ 16;
                 const bool sw = c >= 4;
@@ -322,9 +323,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&bars[V_FULL0 + st]); mbar_arrive(&bars[V8_FREE0 + st]); }
+            if (lane == 0) mbar_arrive(&bars[V_FULL0 + st]);
+            if (++st == V_ST) { st = 0; ph ^= 1; }
+        };
+        uint4 qa[8], qb[8];
+        fetch(qa, 0);
+        fetch(qb, 1);
+        mbar_wait(&bars[Q_READY], 0, abort_flag, p.status, QW_ST_MMA_TIMEOUT);     // the Q tile was staged here
+        for (int pg = 0; pg < n_pg; pg += 2) {
+            put(qa, pg);
+            fetch(qa, pg + 2);
+            put(qb, pg + 1);
+            fetch(qb, pg + 3);
         }
-    } else {
+    } else if (warp < 8) {
         // ---------------- softmax + epilogue ----------------
         const int wg = warp >> 2;
         const int row_l = (warp & 3) * 32 + lane;

@@ -2120,7 +2120,7 @@ bool kv8_prefill(qw_cmd c, const Kv8Call &a, const void *q, void *out, const voi
     Kv8PrefillParams p;
     memset(&p, 0, sizeof p);
     const int32_t end = a.base_pos + rows;
-    if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &p.kc, &p.kmap, 64) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &p.vc, &p.vmap, 64)) return false;
+    if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &p.kc, &p.kmap, 64) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &p.vc, nullptr)) return false;
     p.gqa = q_heads / kv_heads;
     p.tile_rows = 128 / p.gqa;
     if (!encode_heads_map(&p.qmap, q, rows, q_heads, QW_HEAD_DIM, p.gqa, p.tile_rows) || !encode_heads_map(&p.omap, out, rows, q_heads, QW_HEAD_DIM, p.gqa, p.tile_rows) ||
