@@ -128,6 +128,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
           "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
           "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -151,6 +154,9 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, int32_t x, int32_t y, int32_t z, const void *src) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap *map, int32_t x, int32_t y, int32_t z) {
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(x), "r"(y), "r"(z) : "memory");
 }
 __device__ __forceinline__ void bulk_store(void *dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
@@ -222,6 +228,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
                     tma_load_2d(dst + b * KBOX, &p.kmap, b * 128, r, &bars[K_FULL0 + st]);
                     tma_load_2d(dst + b * KBOX + KBOX / 2, &p.kmap, b * 128, r + 64, &bars[K_FULL0 + st]);
                 }
+                // (the gate is wanted at the very end, with nothing left to hide a trip to memory)
+                if (j == 0 && gated)
+                    for (int b = 0; b < 4; b++) prefetch_3d(&p.gmap, b * 64, kvh * p.gqa, r0);
             }
             if (gated) {
                 // the gate tile, into the K stages: both are idle once the last Q K^T has completed
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
             const uint8_t *q_row = smem + OFF_STAGE_Q + 2 * wg * IO_BOX + row_l * 128;
             mbar_wait(&bars[Q_FULL], 0, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
             float mx = 0.0f;
-#pragma unroll
+#pragma unroll 4
             for (int e = 0; e < 16; e++) {
                 const uint4 x = *reinterpret_cast<const uint4 *>(q_row + (e >> 3) * IO_BOX + (((e & 7) ^ sw) << 4));
                 const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
@@ -368,9 +377,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
             sc_row = fabsf(p.scale) * LOG2E * pow2f(k - 7);
             const float fs = p.scale < 0.0f ? -f : f;
             uint8_t *lo_row = smem + OFF_QLO + wg * IO_BOX + row_l * 128;
-#pragma unroll
+#pragma unroll 2
             for (int e = 0; e < 8; e++) {                              // 16 dims: four columns of high parts, a piece of low parts
-                uint32_t lo4[4];
+                uint32_t hi4[4], lo4[4];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const uint4 x = *reinterpret_cast<const uint4 *>(q_row + (e >> 2) * IO_BOX + ((((e & 3) * 2 + h) ^ sw) << 4));
@@ -386,13 +395,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
                         const uint32_t h01 = e4m3x2(a[0], a[1]), h23 = e4m3x2(a[2], a[3]);
                         const uint32_t w01 = f16x2_of(h01), w23 = f16x2_of(h23);
                         const float2 b01 = __half22float2(*reinterpret_cast<const __half2 *>(&w01)), b23 = __half22float2(*reinterpret_cast<const __half2 *>(&w23));
-                        v[e * 4 + h * 2 + i] = h01 | (h23 << 16);
+                        hi4[h * 2 + i] = h01 | (h23 << 16);
                         lo4[h * 2 + i] = e4m3x2(a[0] - b01.x, a[1] - b01.y) | (e4m3x2(a[2] - b23.x, a[3] - b23.y) << 16);
                     }
                 }
                 *reinterpret_cast<uint4 *>(lo_row + ((e ^ sw) << 4)) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+                tmem_st4(t_q + lane_base + wg * 32 + e * 4, hi4);
             }
-            tmem_st32(t_q + lane_base + wg * 32, v);
             fence_proxy_async();                                       // the low parts are read by the tensor core
             tmem_wait_st();
             tc_fence_before();
