@@ -75,7 +75,7 @@ constexpr float NEG_BIG = -1.0e30f;
 constexpr float RESCALE_AT = 8.0f;                    // log2 units
 
 enum Bar { Q_READY = 0, Q_FULL, G_FULL, K_FULL0, K_FULL1, K_FREE0, K_FREE1, V_FULL0, V_FULL1, V_FREE0, V_FREE1,
-           S_READY, S_FREE, P_READY, PV_DONE, PV_ISSUED, V_TAIL, N_BARS };
+           S_READY, S_FREE, P_READY, PV_DONE, PV_ISSUED0, PV_ISSUED1, V_TAIL, N_BARS };
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -314,8 +314,11 @@ __global__ void __launch_bounds__(THREADS, 1) qw_attn_prefill_kernel(const __gri
                 if (j > 0) mbar_wait_hot(&bars[S_FREE], (j - 1) & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
                 // P V of step j-2 goes into the tensor queue first: queued side by side the two
                 // products share the pipe, and the softmax threads wait for the end of P V before
-                // they may write the next P -- which they then do under this product.
-                if (QK_AFTER_PV && j > 1) mbar_wait_hot(&bars[PV_ISSUED], j & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
+                // they may write the next P -- which they then do under this product.  (One barrier for the even and
+                // one for the odd steps: where the K tile of this step came late, P V of step j-1 has been queued too,
+                // and a barrier that every step signals would be a phase ahead of the parity asked for -- for good.)
+                if (QK_AFTER_PV && j > 1)
+                    mbar_wait_hot(&bars[PV_ISSUED0 + (j & 1)], ((j >> 1) - 1) & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
                 tc_fence_after();
                 const uint32_t k_lo = desc_lo(k_a + st * K_BYTES, 16);
                 // A: 16 dims of Q = 8 TMEM columns for dims 0-127, 32 bytes inside the swizzle atom of a
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1) qw_attn_prefill_kernel(const __gri
                     tc_commit(&bars[V_FREE0 + h]);
                 }
                 tc_commit(&bars[PV_DONE]);
-                if (QK_AFTER_PV) mbar_arrive(&bars[PV_ISSUED]);
+                if (QK_AFTER_PV) mbar_arrive(&bars[PV_ISSUED0 + (j & 1)]);
             }
         }
     } else {
