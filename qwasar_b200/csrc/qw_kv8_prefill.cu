@@ -52,7 +52,7 @@ constexpr float NEG_BIG = -1.0e30f;
 constexpr float RESCALE_AT = 8.0f, P_SHIFT = 7.0f;
 
 enum Bar { Q_READY = 0, Q_FULL, G_FULL, K_FULL0, K_FULL1, K_FREE0, K_FREE1, V_FULL0, V_FULL1, V_FULL2, V_FREE0, V_FREE1, V_FREE2,
-           S_READY, S_FREE, P_READY, PV_DONE, PV_ISSUED, N_BARS };
+           S_READY, S_FREE, P_READY, PV_DONE, PV_ISSUED0, PV_ISSUED1, N_BARS };
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -65,10 +65,19 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+__device__ __forceinline__ uint32_t e4m3x2_of_f16(uint32_t v) {
     uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
     return r;
+}
+// a * sigmoid(g), b * sigmoid(h): two exponentials and one reciprocal (the unit that works them out delivers 16 a clock,
+// and the output tile has 32 768 elements).  Gates below -43 count as -43: 2e-19.
+__device__ __forceinline__ void gate2(float &a, float &b, float g, float h) {
+    const float u = 1.0f + __expf(-fmaxf(g, -43.0f)), v = 1.0f + __expf(-fmaxf(h, -43.0f));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * v));
+    a *= r * v;
+    b *= r * u;
 }
 __device__ __forceinline__ uint32_t f16x2_of(uint32_t codes16) {
     uint32_t r;
@@ -162,6 +171,106 @@ __device__ __forceinline__ void bulk_store(void *dst, const void *src, uint32_t 
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
 }
 
+// Q of one thread: 128 dims (half wg) of tile row row_l, from the staged bf16 tile to the two e4m3 parts -- the high one in
+// tensor memory, the low one in shared memory.  Returns scale * log2(e) * the row's power of two.  (A function of its own,
+// not inlined: together with it the compiler orders the softmax loop 3 to 8 % slower.)
+__device__ __noinline__ float stage_q(const Kv8PrefillParams &p, uint8_t *smem, uint64_t *bars, volatile int *abort_flag, float *xch, uint32_t t_q, int wg,
+                                      int row_l, bool in_tile, uint32_t lane_base, int lane) {
+    const uint32_t sw = row_l & 7;
+    // this thread's 128 dims of its row: largest magnitude (with the other half's), then the two e4m3 parts
+    const uint8_t *q_row = smem + OFF_STAGE_Q + 2 * wg * IO_BOX + row_l * 128;
+    mbar_wait(&bars[Q_FULL], 0, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+    // (held in registers: read again between the stores below, each piece would wait for the one before it)
+    uint4 x[16];
+    uint32_t big = 0;                                          // magnitudes of bf16 order like their bits
+#pragma unroll
+    for (int e = 0; e < 16; e++) x[e] = *reinterpret_cast<const uint4 *>(q_row + (e >> 3) * IO_BOX + (((e & 7) ^ sw) << 4));
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+        big = __vmaxu2(__vmaxu2(big, x[e].x & 0x7fff7fffu), __vmaxu2(x[e].y & 0x7fff7fffu, __vmaxu2(x[e].z & 0x7fff7fffu, x[e].w & 0x7fff7fffu)));
+    float mx = __uint_as_float(max(big & 0xffff0000u, big << 16));
+    xch[wg * BM + row_l] = mx;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    mx = in_tile ? fmaxf(mx, xch[(wg ^ 1) * BM + row_l]) : 0.0f;
+    const int k = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 100);     // scaled below 2^8
+    const float f = in_tile ? pow2f(7 - k) : 0.0f;
+    const float sc_row = fabsf(p.scale) * LOG2E * pow2f(k - 7);
+    const float fs = p.scale < 0.0f ? -f : f;
+    uint8_t *lo_row = smem + OFF_QLO + wg * IO_BOX + row_l * 128;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {                              // 16 dims: four columns of high parts, a piece of low parts
+        uint32_t hi4[4], lo4[4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t xw[4] = {x[2 * e + h].x, x[2 * e + h].y, x[2 * e + h].z, x[2 * e + h].w};
+            uint32_t hc[4], lc[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // (eight significant bits fit fp16, so the difference to the high part is exact there)
+                const float a0 = in_tile ? __uint_as_float(xw[i] << 16) * fs : 0.0f, a1 = in_tile ? __uint_as_float(xw[i] & 0xffff0000u) * fs : 0.0f;
+                const uint32_t a = pack_f16(a0, a1);
+                hc[i] = e4m3x2_of_f16(a);
+                const uint32_t w = f16x2_of(hc[i]);
+                const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&w));
+                lc[i] = e4m3x2_of_f16(*reinterpret_cast<const uint32_t *>(&d));
+            }
+            hi4[h * 2] = hc[0] | (hc[1] << 16); hi4[h * 2 + 1] = hc[2] | (hc[3] << 16);
+            lo4[h * 2] = lc[0] | (lc[1] << 16); lo4[h * 2 + 1] = lc[2] | (lc[3] << 16);
+        }
+        *reinterpret_cast<uint4 *>(lo_row + ((e ^ sw) << 4)) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+        tmem_st4(t_q + lane_base + wg * 32 + e * 4, hi4);
+    }
+    fence_proxy_async();                                       // the low parts are read by the tensor core
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[Q_READY]);
+    asm volatile("bar.sync 1, 256;" ::: "memory");             // (xch is written again below)
+    return sc_row;
+}
+
+// The 128 softmax threads of half wg, with what they wrote to shared memory in view of the copy engine.
+__device__ __forceinline__ void half_sync(int wg) {
+    fence_proxy_async();
+    if (wg == 0) asm volatile("bar.sync 2, 128;" ::: "memory");
+    else asm volatile("bar.sync 3, 128;" ::: "memory");
+}
+
+// The finished tile of one thread: 128 dims of its row, divided by the denominator, gated, into the output boxes.
+__device__ __noinline__ void finish_tile(const Kv8PrefillParams &p, uint8_t *smem, uint64_t *bars, volatile int *abort_flag, uint32_t t_o, int wg, int row_l,
+                                         uint32_t lane_base, bool elected, bool gated, float l, int kvh, int r0) {
+    const uint32_t sw = row_l & 7;
+    uint8_t *io_row = smem + OFF_STAGE_IO + row_l * 128;
+    uint32_t v[32];
+    if (gated) mbar_wait(&bars[G_FULL], 0, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+    const float inv = 1.0f / l;
+#pragma unroll 1
+    for (int c = 4 * wg; c < 4 * wg + 4; c++) {        // 32 outputs = 64 bytes = half a box row
+        tmem_ld32(t_o + lane_base + c * 32, v);
+        uint4 *bx = reinterpret_cast<uint4 *>(io_row + (c >> 1) * IO_BOX);
+        uint4 gt[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) gt[k] = gated ? bx[((c & 1) * 4 + k) ^ sw] : make_uint4(0, 0, 0, 0);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = __uint_as_float(v[k * 8 + e]) * inv;
+            if (gated) {
+                const uint32_t gw[4] = {gt[k].x, gt[k].y, gt[k].z, gt[k].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) gate2(o[2 * e], o[2 * e + 1], __uint_as_float(gw[e] << 16), __uint_as_float(gw[e] & 0xffff0000u));
+            }
+            bx[((c & 1) * 4 + k) ^ sw] = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
+        }
+        if (c & 1) {
+            half_sync(wg);
+            if (elected) { tma_store_3d(&p.omap, (c >> 1) * 64, kvh * p.gqa, r0, smem + OFF_STAGE_IO + (c >> 1) * IO_BOX); tma_store_commit(); }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_constant__ Kv8PrefillParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {                      // swizzled boxes need 1024-byte alignment
@@ -213,91 +322,98 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
         return max(id, 0) * QW_KV8_PAGE_TOKENS;
     };
 
-    if (warp == W_K) {
-        if (lane == 0) {
-            mbar_expect_tx(&bars[Q_FULL], 4 * p.box_bytes);
-            for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_Q + b * IO_BOX, &p.qmap, b * 64, kvh * p.gqa, r0, &bars[Q_FULL]);
-            for (int j = 0; j < n_t; j++) {
-                const int st = j & 1;
-                const int32_t r = step_row(p.kc, j);
-                if (j >= 2) mbar_wait(&bars[K_FREE0 + st], ((j >> 1) - 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
-                mbar_expect_tx(&bars[K_FULL0 + st], K_BYTES);
-                uint8_t *dst = smem + OFF_K + st * K_BYTES;
+    // Registers follow the work (per warpgroup; 2 x 168 + 64 + 112 = 4 x 128, what the block was launched with).
+    if (warp >= 8 && warp < W_CV) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == W_K) {
+            if (lane == 0) {
+                mbar_expect_tx(&bars[Q_FULL], 4 * p.box_bytes);
+                for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_Q + b * IO_BOX, &p.qmap, b * 64, kvh * p.gqa, r0, &bars[Q_FULL]);
+                for (int j = 0; j < n_t; j++) {
+                    const int st = j & 1;
+                    const int32_t r = step_row(p.kc, j);
+                    if (j >= 2) mbar_wait(&bars[K_FREE0 + st], ((j >> 1) - 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
+                    mbar_expect_tx(&bars[K_FULL0 + st], K_BYTES);
+                    uint8_t *dst = smem + OFF_K + st * K_BYTES;
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    tma_load_2d(dst + b * KBOX, &p.kmap, b * 128, r, &bars[K_FULL0 + st]);
-                    tma_load_2d(dst + b * KBOX + KBOX / 2, &p.kmap, b * 128, r + 64, &bars[K_FULL0 + st]);
-                }
-                // (the gate is wanted at the very end, with nothing left to hide a trip to memory)
-                if (j == 0 && gated)
-                    for (int b = 0; b < 4; b++) prefetch_3d(&p.gmap, b * 64, kvh * p.gqa, r0);
-            }
-            if (gated) {
-                // the gate tile, into the K stages: both are idle once the last Q K^T has completed
-                mbar_wait(&bars[K_FREE0 + ((n_t - 1) & 1)], ((n_t - 1) >> 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
-                mbar_expect_tx(&bars[G_FULL], 4 * p.box_bytes);
-                for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_IO + b * IO_BOX, &p.gmap, b * 64, kvh * p.gqa, r0, &bars[G_FULL]);
-            }
-        }
-    } else if (warp == W_MMA) {
-        if (lane == 0) {
-            constexpr uint32_t idesc_qk = instr_desc(128, BN, 0);
-            constexpr uint32_t hi = desc_hi(1024);
-            const uint32_t k_a = smem_u32(smem + OFF_K);
-            const uint32_t ql = desc_lo(smem_u32(smem + OFF_QLO), 16);
-            mbar_wait(&bars[Q_READY], 0, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
-            for (int j = 0; j < n_t; j++) {
-                const int st = j & 1;
-                mbar_wait_hot(&bars[K_FULL0 + st], (j >> 1) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-                if (j > 0) mbar_wait_hot(&bars[S_FREE], (j - 1) & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
-                // P V of step j-2 goes into the tensor queue first (the softmax threads wait for its end)
-                if (j > 1) mbar_wait_hot(&bars[PV_ISSUED], j & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
-                tc_fence_after();
-                const uint32_t k_lo = desc_lo(k_a + st * K_BYTES, 16);
-                // 32 dims a product: 8 columns of Q high, 32 bytes inside the swizzle atom of Q low and K
-#pragma unroll
-                for (int ks = 0; ks < 8; ks++) {
-                    const uint32_t kd = k_lo + (ks >> 2) * (KBOX >> 4) + (ks & 3) * 2;
-                    mma_ts_f8(ks > 0, t_s, t_q + ks * 8, kd, hi, idesc_qk);
-                }
-#pragma unroll
-                for (int ks = 0; ks < 8; ks++) {
-                    const uint32_t kd = k_lo + (ks >> 2) * (KBOX >> 4) + (ks & 3) * 2;
-                    mma_ss_f8(true, t_s, ql + (ks >> 2) * (IO_BOX >> 4) + (ks & 3) * 2, hi, kd, hi, idesc_qk);
-                }
-                tc_commit(&bars[S_READY]);
-                tc_commit(&bars[K_FREE0 + st]);
-            }
-        }
-    } else if (warp == W_PV) {
-        if (lane == 0) {
-            constexpr uint32_t idesc_pv = instr_desc(128, 256, 1);
-            constexpr uint32_t hi = desc_hi(1024);
-            const uint32_t v_a = smem_u32(smem + OFF_V);
-            int st = 0;
-            uint32_t ph = 0;                                 // stage and parity of the next 64 keys
-            for (int j = 0; j < n_t; j++) {
-                mbar_wait_hot(&bars[V_FULL0 + st], ph, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-                mbar_wait_hot(&bars[P_READY], j & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
-                tc_fence_after();
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if (h == 1) {
-                        mbar_wait_hot(&bars[V_FULL0 + st], ph, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-                        tc_fence_after();
+                    for (int b = 0; b < 2; b++) {
+                        tma_load_2d(dst + b * KBOX, &p.kmap, b * 128, r, &bars[K_FULL0 + st]);
+                        tma_load_2d(dst + b * KBOX + KBOX / 2, &p.kmap, b * 128, r + 64, &bars[K_FULL0 + st]);
                     }
-                    const uint32_t v_lo = desc_lo(v_a + st * V_BYTES, VBOX);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ks++)       // 16 keys: 8 columns of P, 2048 bytes of V
-                        mma_ts_f16(j > 0 || h > 0 || ks > 0, t_o, t_p + (h * 4 + ks) * 8, v_lo + ks * 128, hi, idesc_pv);
-                    tc_commit(&bars[V_FREE0 + st]);
-                    if (++st == V_ST) { st = 0; ph ^= 1; }
+                    // (the gate is wanted at the very end, with nothing left to hide a trip to memory)
+                    if (j == 0 && gated)
+                        for (int b = 0; b < 4; b++) prefetch_3d(&p.gmap, b * 64, kvh * p.gqa, r0);
                 }
-                tc_commit(&bars[PV_DONE]);
-                mbar_arrive(&bars[PV_ISSUED]);
+                if (gated) {
+                    // the gate tile, into the K stages: both are idle once the last Q K^T has completed
+                    mbar_wait(&bars[K_FREE0 + ((n_t - 1) & 1)], ((n_t - 1) >> 1) & 1, abort_flag, p.status, QW_ST_SLOT_TIMEOUT);
+                    mbar_expect_tx(&bars[G_FULL], 4 * p.box_bytes);
+                    for (int b = 0; b < 4; b++) tma_load_3d(smem + OFF_STAGE_IO + b * IO_BOX, &p.gmap, b * 64, kvh * p.gqa, r0, &bars[G_FULL]);
+                }
+            }
+        } else if (warp == W_MMA) {
+            if (lane == 0) {
+                constexpr uint32_t idesc_qk = instr_desc(128, BN, 0);
+                constexpr uint32_t hi = desc_hi(1024);
+                const uint32_t k_a = smem_u32(smem + OFF_K);
+                const uint32_t ql = desc_lo(smem_u32(smem + OFF_QLO), 16);
+                mbar_wait(&bars[Q_READY], 0, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
+                for (int j = 0; j < n_t; j++) {
+                    const int st = j & 1;
+                    mbar_wait_hot(&bars[K_FULL0 + st], (j >> 1) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+                    if (j > 0) mbar_wait_hot(&bars[S_FREE], (j - 1) & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
+                    // P V of step j-2 goes into the tensor queue first (the softmax threads wait for its end).  One
+                    // barrier for the even and one for the odd steps: where the K tile of this step came late, P V of
+                    // step j-1 has been queued too, and one barrier would be a phase ahead of the parity asked for.
+                    if (j > 1) mbar_wait_hot(&bars[PV_ISSUED0 + (j & 1)], ((j >> 1) - 1) & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
+                    tc_fence_after();
+                    const uint32_t k_lo = desc_lo(k_a + st * K_BYTES, 16);
+                    // 32 dims a product: 8 columns of Q high, 32 bytes inside the swizzle atom of Q low and K
+#pragma unroll
+                    for (int ks = 0; ks < 8; ks++) {
+                        const uint32_t kd = k_lo + (ks >> 2) * (KBOX >> 4) + (ks & 3) * 2;
+                        mma_ts_f8(ks > 0, t_s, t_q + ks * 8, kd, hi, idesc_qk);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 8; ks++) {
+                        const uint32_t kd = k_lo + (ks >> 2) * (KBOX >> 4) + (ks & 3) * 2;
+                        mma_ss_f8(true, t_s, ql + (ks >> 2) * (IO_BOX >> 4) + (ks & 3) * 2, hi, kd, hi, idesc_qk);
+                    }
+                    tc_commit(&bars[S_READY]);
+                    tc_commit(&bars[K_FREE0 + st]);
+                }
+            }
+        } else if (warp == W_PV) {
+            if (lane == 0) {
+                constexpr uint32_t idesc_pv = instr_desc(128, 256, 1);
+                constexpr uint32_t hi = desc_hi(1024);
+                const uint32_t v_a = smem_u32(smem + OFF_V);
+                int st = 0;
+                uint32_t ph = 0;                                 // stage and parity of the next 64 keys
+                for (int j = 0; j < n_t; j++) {
+                    mbar_wait_hot(&bars[V_FULL0 + st], ph, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+                    mbar_wait_hot(&bars[P_READY], j & 1, abort_flag, p.status, QW_ST_MMA_TIMEOUT);
+                    tc_fence_after();
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (h == 1) {
+                            mbar_wait_hot(&bars[V_FULL0 + st], ph, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+                            tc_fence_after();
+                        }
+                        const uint32_t v_lo = desc_lo(v_a + st * V_BYTES, VBOX);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ks++)       // 16 keys: 8 columns of P, 2048 bytes of V
+                            mma_ts_f16(j > 0 || h > 0 || ks > 0, t_o, t_p + (h * 4 + ks) * 8, v_lo + ks * 128, hi, idesc_pv);
+                        tc_commit(&bars[V_FREE0 + st]);
+                        if (++st == V_ST) { st = 0; ph ^= 1; }
+                    }
+                    tc_commit(&bars[PV_DONE]);
+                    mbar_arrive(&bars[PV_ISSUED0 + (j & 1)]);
+                }
             }
         }
     } else if (warp >= W_CV) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
         // ---------------- V codes -> fp16 ----------------
         // Eight lanes take the eight 16-byte pieces (16 dims) of half a code row, which become two 16-byte pieces of the
         // fp16 row each; lanes 4-7 of the eight write their second piece first, so that a store meets all banks.  The
@@ -345,7 +461,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
             put(qb, pg + 1);
             fetch(qb, pg + 3);
         }
-    } else if (warp < 8) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         // ---------------- softmax + epilogue ----------------
         const int wg = warp >> 2;
         const int row_l = (warp & 3) * 32 + lane;
@@ -355,60 +472,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         float *xch = reinterpret_cast<float *>(smem + OFF_XCH);         // [2][2][BM]
         const uint32_t sw = row_l & 7;
-        float sc_row;
+        const float sc_row = stage_q(p, smem, bars, abort_flag, xch, t_q, wg, row_l, in_tile, lane_base, lane);
         uint32_t v[32];
-        {
-            // this thread's 128 dims of its row: largest magnitude (with the other half's), then the two e4m3 parts
-            const uint8_t *q_row = smem + OFF_STAGE_Q + 2 * wg * IO_BOX + row_l * 128;
-            mbar_wait(&bars[Q_FULL], 0, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-            float mx = 0.0f;
-#pragma unroll 4
-            for (int e = 0; e < 16; e++) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(q_row + (e >> 3) * IO_BOX + (((e & 7) ^ sw) << 4));
-                const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(xw[i] << 16)), fabsf(__uint_as_float(xw[i] & 0xffff0000u))));
-            }
-            xch[wg * BM + row_l] = mx;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            mx = in_tile ? fmaxf(mx, xch[(wg ^ 1) * BM + row_l]) : 0.0f;
-            const int k = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 100);     // scaled below 2^8
-            const float f = in_tile ? pow2f(7 - k) : 0.0f;
-            sc_row = fabsf(p.scale) * LOG2E * pow2f(k - 7);
-            const float fs = p.scale < 0.0f ? -f : f;
-            uint8_t *lo_row = smem + OFF_QLO + wg * IO_BOX + row_l * 128;
-#pragma unroll 2
-            for (int e = 0; e < 8; e++) {                              // 16 dims: four columns of high parts, a piece of low parts
-                uint32_t hi4[4], lo4[4];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(q_row + (e >> 2) * IO_BOX + ((((e & 3) * 2 + h) ^ sw) << 4));
-                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        float a[4];
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            a[2 * c] = in_tile ? __uint_as_float(xw[2 * i + c] << 16) * fs : 0.0f;
-                            a[2 * c + 1] = in_tile ? __uint_as_float(xw[2 * i + c] & 0xffff0000u) * fs : 0.0f;
-                        }
-                        const uint32_t h01 = e4m3x2(a[0], a[1]), h23 = e4m3x2(a[2], a[3]);
-                        const uint32_t w01 = f16x2_of(h01), w23 = f16x2_of(h23);
-                        const float2 b01 = __half22float2(*reinterpret_cast<const __half2 *>(&w01)), b23 = __half22float2(*reinterpret_cast<const __half2 *>(&w23));
-                        hi4[h * 2 + i] = h01 | (h23 << 16);
-                        lo4[h * 2 + i] = e4m3x2(a[0] - b01.x, a[1] - b01.y) | (e4m3x2(a[2] - b23.x, a[3] - b23.y) << 16);
-                    }
-                }
-                *reinterpret_cast<uint4 *>(lo_row + ((e ^ sw) << 4)) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-                tmem_st4(t_q + lane_base + wg * 32 + e * 4, hi4);
-            }
-            fence_proxy_async();                                       // the low parts are read by the tensor core
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[Q_READY]);
-            asm volatile("bar.sync 1, 256;" ::: "memory");             // (xch is written again below)
-        }
         float m = NEG_BIG, l = 0.0f;
         const uint32_t p_cols = t_p + lane_base + wg * 32;
         const uint8_t *ke = p.kc.exps + (size_t)kvh * p.kc.exp_stride, *ve = p.vc.exps + (size_t)kvh * p.vc.exp_stride;
@@ -504,15 +569,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
         tc_fence_after();
         const bool elected = (warp & 3) == 0 && lane == 0;
         uint8_t *io_row = smem + OFF_STAGE_IO + row_l * 128;
-        auto half_sync = [&]() {
-            fence_proxy_async();
-            if (wg == 0) asm volatile("bar.sync 2, 128;" ::: "memory");
-            else asm volatile("bar.sync 3, 128;" ::: "memory");
-        };
         if (!whole) {
             // a share's sums: boxes of 32 dims x 128 rows as they lie in shared memory, (m, l) beside them
             if (wg == 0) stat[row_l] = make_float2(m, l);
             uint8_t *dst = reinterpret_cast<uint8_t *>(p.pacc) + (size_t)item * (8 * IO_BOX);
+            const uint32_t used = (uint32_t)(min(p.tile_rows, p.rows - r0) * p.gqa) * 128;      // (tile rows past the call's end: not written)
 #pragma unroll 1
             for (int c = 4 * wg; c < 4 * wg + 4; c++) {
                 tmem_ld32(t_o + lane_base + c * 32, v);
@@ -520,50 +581,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_prefill_kernel(const __grid_co
 #pragma unroll
                 for (int k = 0; k < 8; k++)
                     *reinterpret_cast<uint4 *>(io_row + c * IO_BOX + ((k ^ sw) << 4)) = make_uint4(v[k * 4], v[k * 4 + 1], v[k * 4 + 2], v[k * 4 + 3]);
-                half_sync();
-                if (elected) { bulk_store(dst + c * IO_BOX, smem + OFF_STAGE_IO + c * IO_BOX, IO_BOX); tma_store_commit(); }
+                half_sync(wg);
+                if (elected) { bulk_store(dst + c * IO_BOX, smem + OFF_STAGE_IO + c * IO_BOX, used); tma_store_commit(); }
             }
         } else {
-            if (gated) mbar_wait(&bars[G_FULL], 0, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-            const float inv = 1.0f / l;
-#pragma unroll 1
-            for (int c = 4 * wg; c < 4 * wg + 4; c++) {        // 32 outputs = 64 bytes = half a box row
-                tmem_ld32(t_o + lane_base + c * 32, v);
-                tmem_wait_ld();
-                uint8_t *bx = io_row + (c >> 1) * IO_BOX;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    uint4 *slot = reinterpret_cast<uint4 *>(bx + ((((c & 1) * 4 + k) ^ sw) << 4));
-                    float o[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) o[e] = __uint_as_float(v[k * 8 + e]) * inv;
-                    if (gated) {
-                        const uint4 g = *slot;
-                        const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            o[2 * e] = __fdividef(o[2 * e], 1.0f + __expf(-__uint_as_float(gw[e] << 16)));
-                            o[2 * e + 1] = __fdividef(o[2 * e + 1], 1.0f + __expf(-__uint_as_float(gw[e] & 0xffff0000u)));
-                        }
-                    }
-                    *slot = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
-                }
-                if (c & 1) {
-                    half_sync();
-                    if (elected) { tma_store_3d(&p.omap, (c >> 1) * 64, kvh * p.gqa, r0, smem + OFF_STAGE_IO + (c >> 1) * IO_BOX); tma_store_commit(); }
-                }
-            }
+            finish_tile(p, smem, bars, abort_flag, t_o, wg, row_l, lane_base, elected, gated, l, kvh, r0);
         }
         if (elected) tma_store_wait_read();                   // shared memory must outlive the copies
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {                                    // a wait gave up: copies and products of this CTA may still be under way
+        for (int i = 0; i < 4096; i++) __nanosleep(10000);
+        __syncthreads();
+    }
     if (warp == W_MMA) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (*abort_flag)                                      // a wait gave up: copies of this CTA may still be under way
-        for (int i = 0; i < 4096; i++) __nanosleep(10000);
 }
 
 // Adds up the shares of a tile.  A block takes 4 / SL rows of the output (a row: one head of one row of the call), SL
@@ -627,8 +662,8 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
     float o[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
     if (p.gate) {
         const uint2 g = *reinterpret_cast<const uint2 *>(p.gate + (size_t)rh * p.gate_stride + d4);
-        o[0] = __fdividef(o[0], 1.0f + __expf(-__uint_as_float(g.x << 16))); o[1] = __fdividef(o[1], 1.0f + __expf(-__uint_as_float(g.x & 0xffff0000u)));
-        o[2] = __fdividef(o[2], 1.0f + __expf(-__uint_as_float(g.y << 16))); o[3] = __fdividef(o[3], 1.0f + __expf(-__uint_as_float(g.y & 0xffff0000u)));
+        gate2(o[0], o[1], __uint_as_float(g.x << 16), __uint_as_float(g.x & 0xffff0000u));
+        gate2(o[2], o[3], __uint_as_float(g.y << 16), __uint_as_float(g.y & 0xffff0000u));
     }
     *reinterpret_cast<uint2 *>(p.out + (size_t)rh * 256 + d4) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
 }
