@@ -635,21 +635,26 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
 // =======================================================================================
 // NT tiles of eight query rows.  Two warps share a tile of 32 keys: each scores 16 of its keys against all rows (the K
 // codes are widened once, however many rows there are) and each takes 128 dims of V for all 32 keys.  What they swap is
-// the weights, through shared memory, one barrier of the pair per tile: each weighs its keys against its own running
-// maximum, a whole number, so that the other can bring the weights to the common maximum by an exact power of two.
+// the weights, through shared memory.  The running maximum is the pair's and lags: it moves only when a score exceeds it
+// by more than 2^4 (the pair votes with the barrier that also guards the weights' buffer), so that most tiles need no
+// reduction over the lanes and no rescaling; the weights reach 2^15 then, which fp16 holds.
+constexpr float VF_LAG = 4.0f, VF_SHIFT = 11.0f;
+
 template <int NT, bool F32>
 struct VfCfg {
     static constexpr int WARPS = NT == 4 ? 8 : 12, PAIRS = WARPS / 2, THREADS = WARPS * 32;
-    static constexpr int NS = NT == 4 ? 4 : 3;                  // 4 KB slots of a warp: its part of K or V of a tile
+    static constexpr int VS = F32 && NT == 3 ? 1 : 2, NS = 2 + VS;       // 4 KB slots of a warp: two for its part of K, VS for its part of V
     static constexpr int PX = NT * 32 * (F32 ? 16 : 8);         // weights of one warp's keys, as B fragments
+    static constexpr int ROWS = NT * 8;
     static constexpr int OFF_Q = WARPS * NS * 4096;
-    static constexpr int OFF_PX = OFF_Q + NT * (F32 ? 8192 : 4096);       // [pair][tile parity][half]
-    static constexpr int OFF_MX = OFF_PX + PAIRS * 4 * PX;      // [pair][tile parity][half][NT * 8]
-    static constexpr int OFF_M = OFF_MX + PAIRS * 4 * NT * 32;  // [warp][NT * 8]
-    static constexpr int OFF_L = OFF_M + WARPS * NT * 32;
-    static constexpr int OFF_SC = OFF_L + WARPS * NT * 32;      // [NT * 8]
-    static constexpr int OFF_LIM = OFF_SC + NT * 32;            // [NT * 8] last key of a row
-    static constexpr int OFF_BAR = OFF_LIM + NT * 32;           // full[warp][slot], abort
+    static constexpr int OFF_PX = OFF_Q + NT * (F32 ? 8192 : 4096);       // [pair][half]
+    static constexpr int OFF_MX = OFF_PX + WARPS * PX;          // [warp][ROWS] maxima of a tile
+    static constexpr int OFF_M = OFF_MX + WARPS * ROWS * 4;     // [pair][ROWS], then the pair's factor
+    static constexpr int OFF_L = OFF_M + PAIRS * ROWS * 4;      // [warp][ROWS]
+    static constexpr int OFF_T = OFF_L + WARPS * ROWS * 4;      // [2][ROWS] maximum and sum of all pairs
+    static constexpr int OFF_SC = OFF_T + 2 * ROWS * 4;         // [ROWS]
+    static constexpr int OFF_LIM = OFF_SC + ROWS * 4;           // [ROWS] last key of a row
+    static constexpr int OFF_BAR = OFF_LIM + ROWS * 4;          // full[warp][slot], abort
     static constexpr int SMEM = OFF_BAR + WARPS * NS * 8 + 16;
     static_assert(SMEM <= 232448, "exceeds the 227 KB a CTA may use");
     static_assert(NT <= NS, "a warp's sums do not fit its slots");
@@ -658,10 +663,11 @@ struct VfCfg {
 template <int NT, bool F32>
 __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(const __grid_constant__ Kv8AttnParams p) {
     using Cfg = VfCfg<NT, F32>;
-    constexpr int NS = Cfg::NS, PAIRS = Cfg::PAIRS, ROWS = NT * 8;
+    constexpr int NS = Cfg::NS, VS = Cfg::VS, PAIRS = Cfg::PAIRS, ROWS = Cfg::ROWS;
     extern __shared__ __align__(1024) uint8_t smem[];
     float *sm_m = reinterpret_cast<float *>(smem + Cfg::OFF_M);
     float *sm_l = reinterpret_cast<float *>(smem + Cfg::OFF_L);
+    float *sm_t = reinterpret_cast<float *>(smem + Cfg::OFF_T);
     float *sm_sc = reinterpret_cast<float *>(smem + Cfg::OFF_SC);
     int *sm_lim = reinterpret_cast<int *>(smem + Cfg::OFF_LIM);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + Cfg::OFF_BAR);
@@ -686,10 +692,12 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
     pdl_launch_next();
 
     uint8_t *ring = smem + warp * NS * 4096;
-    full += warp * NS;
+    uint64_t *full_k = full + warp * NS, *full_v = full_k + 2;
+    uint8_t *px = smem + Cfg::OFF_PX + pair * 2 * Cfg::PX;
+    float *mx = reinterpret_cast<float *>(smem + Cfg::OFF_MX) + pair * 2 * ROWS;
     const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
     Where w = locate(p, lo);
-    uint32_t E0 = 0;                                 // ring entries of this warp before the current segment
+    uint32_t done = 0;                               // tiles of this pair before the current segment
 
     for (int T = lo; T < hi;) {
         const Kv8AttnSeq &sq = p.seq[w.s];
@@ -697,51 +705,60 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
         const int valid = sq.rows * p.gqa, head0 = w.h * p.gqa;
         const int n_keys = sq.base_pos + sq.rows;
         const int nt = pair < seg_n ? (seg_n - pair + PAIRS - 1) / PAIRS : 0;      // this pair's tiles
-        const uint32_t E1 = E0 + 2 * nt;
 
-        int win_k = 0, win_v = 0, win_e = 0;         // code rows and exponents of 32 tiles, one per lane
-        auto window = [&](int i0) {
-            const int i = i0 + lane;
-            if (i < nt) {
-                const int key = (seg_t0 + pair + i * PAIRS) * TILE;
-                const int64_t kr = code_row(sq.kc, w.h, key), vr = code_row(sq.vc, w.h, key);
-                if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
-                win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
-                const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key / BLK]);
-                const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key / BLK]);
-                win_e = (ek & 0xffff) | (ev << 16);
-            }
+        // code rows of 32 tiles, one per lane, looked up two tiles ahead of their use; exponents of 32 tiles
+        int win_k = 0, win_v = 0, win_e = 0;
+        auto key_of = [&](int i) { return (seg_t0 + pair + i * PAIRS) * TILE; };
+        auto rows_from = [&](int i0) {
+            if (i0 + lane >= nt) return;
+            const int64_t kr = code_row(sq.kc, w.h, key_of(i0 + lane)), vr = code_row(sq.vc, w.h, key_of(i0 + lane));
+            if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
+            win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
         };
-        // entry E: K (even) or V (odd) of tile (E - E0) / 2
-        auto load = [&](uint32_t E) {
-            const int i = (int)(E - E0) >> 1, is_v = (int)(E - E0) & 1;
-            if (!is_v && (i & 31) == 0) window(i);
-            const int row = __shfl_sync(0xffffffffu, is_v ? win_v : win_k, i & 31);
+        auto exps_from = [&](int i0) {
+            if (i0 + lane >= nt) return;
+            const int b = key_of(i0 + lane) / BLK;
+            const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + b]), ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + b]);
+            win_e = (ek & 0xffff) | (ev << 16);
+        };
+        // lane 0: this warp's 16 keys x 256 dims of K, and 32 keys x 128 dims of V, of the pair's n-th tile
+        auto load_k = [&](uint32_t n, int row) {
+            uint8_t *dst = ring + (n & 1) * 4096;
+            uint64_t *bar = &full_k[n & 1];
+            mbar_expect_tx(bar, 4096);
+            tma_load_2d(dst, &p.maps[sq.kmap], 0, row + 16 * half, bar);
+            tma_load_2d(dst + 2048, &p.maps[sq.kmap], 128, row + 16 * half, bar);
+        };
+        auto load_v = [&](uint32_t n, int row) {
+            const uint32_t sl = VS == 2 ? n & 1 : 0;
+            uint8_t *dst = ring + (2 + sl) * 4096;
+            mbar_expect_tx(&full_v[sl], 4096);
+            tma_load_2d(dst, &p.maps[sq.vmap], 128 * half, row, &full_v[sl]);
+            tma_load_2d(dst + 2048, &p.maps[sq.vmap], 128 * half, row + 16, &full_v[sl]);
+        };
+        if (nt > 0) {
+            rows_from(0);
+            const int k1 = __shfl_sync(0xffffffffu, win_k, 1), v1 = __shfl_sync(0xffffffffu, win_v, 1);
             if (lane == 0) {
-                const uint32_t slot = E % NS;
-                uint8_t *dst = ring + slot * 4096;
-                mbar_expect_tx(&full[slot], 4096);
-                if (is_v) {                          // 32 keys x this warp's 128 dims
-                    tma_load_2d(dst, &p.maps[sq.vmap], 128 * half, row, &full[slot]);
-                    tma_load_2d(dst + 2048, &p.maps[sq.vmap], 128 * half, row + 16, &full[slot]);
-                } else {                             // this warp's 16 keys x 256 dims
-                    tma_load_2d(dst, &p.maps[sq.kmap], 0, row + 16 * half, &full[slot]);
-                    tma_load_2d(dst + 2048, &p.maps[sq.kmap], 128, row + 16 * half, &full[slot]);
+                load_k(done, win_k);
+                load_v(done, win_v);
+                if (nt > 1) {
+                    load_k(done + 1, k1);
+                    if (VS == 2) load_v(done + 1, v1);
                 }
             }
-        };
-        for (uint32_t E = E0; E < E1 && E < E0 + NS; E++) load(E);
+        }
         for (int row = warp; row < ROWS; row += Cfg::WARPS) stage_q<F32>(p, sq, head0, valid, row, lane, smem + Cfg::OFF_Q, sm_sc + row);
         if (threadIdx.x < ROWS) sm_lim[threadIdx.x] = (int)threadIdx.x < valid ? sq.base_pos + (int)threadIdx.x / p.gqa : n_keys - 1;
         __syncthreads();
 
         float o[NT][8][4];
-        float m[NT][2], l[NT][2], R[NT][2];          // rows 8 n + 2 t and the one after it; R: both halves' maximum
+        float l[NT][2], R[NT][2];                    // rows 8 n + 2 t and the one after it
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
-            m[n][0] = m[n][1] = R[n][0] = R[n][1] = -INFINITY;
+            R[n][0] = R[n][1] = -INFINITY;
             l[n][0] = l[n][1] = 0.0f;
         }
         const uint32_t q_base = smem_u32(smem + Cfg::OFF_Q) + lane * 16;
@@ -750,19 +767,23 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
 #pragma unroll 1
         for (int i = 0; i < nt; i++) {
             const int key0 = (seg_t0 + pair + i * PAIRS) * TILE;
-            const uint32_t EK = E0 + 2 * i, EV = EK + 1;
-            // (the window moves on when the K entry of tile 32 k is asked for, up to two tiles ahead of its use: the
-            // exponents of this tile are read from memory, where the window's lookup has brought them near)
-            const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key0 / BLK]);
-            const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key0 / BLK]);
+            const uint32_t n_t = done + i;
+            if ((i & 31) == 0) exps_from(i);
+            const int ex = __shfl_sync(0xffffffffu, win_e, i & 31);
+            constexpr int AHEAD_V = VS == 2 ? 2 : 1;
+            int nv = __shfl_sync(0xffffffffu, win_v, (i + 1) & 31);
+            if (((i + 2) & 31) == 0) rows_from(i + 2);
+            const int nk = __shfl_sync(0xffffffffu, win_k, (i + 2) & 31);
+            if (VS == 2) nv = __shfl_sync(0xffffffffu, win_v, (i + 2) & 31);
+            const int ek = (int)(int16_t)(ex & 0xffff), ev = ex >> 16;
 
             // ---- S^T = K Q^T for this warp's 16 keys ----
             float s[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            mbar_wait(&full[EK % NS], (EK / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            mbar_wait(&full_k[n_t & 1], (n_t >> 1) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
             {
-                const uint32_t kb = smem_u32(ring + (EK % NS) * 4096) + tok * 128;
+                const uint32_t kb = smem_u32(ring + (n_t & 1) * 4096) + tok * 128;
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     uint32_t kw[2][4];                 // keys tok, tok + 8
@@ -797,13 +818,12 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                 }
             }
             __syncwarp();
-            if (EK + NS < E1) load(EK + NS);
+            if (lane == 0 && i + 2 < nt) load_k(n_t + 2, nk);
 
-            // ---- weights of the 16 keys against this warp's own maximum, a whole number ----
-            const float fk = pow2f(ek), fv = (float)ev, iv = pow2f(-ev);
+            // ---- scores; does any exceed the running maximum by more than it may lag? ----
+            const float fk = pow2f(ek), fv = (float)ev;
             const bool masked = key0 + TILE > sq.base_pos + 1;
-            uint8_t *px = smem + Cfg::OFF_PX + (pair * 4 + (i & 1) * 2) * Cfg::PX;
-            float *mx = reinterpret_cast<float *>(smem + Cfg::OFF_MX) + (pair * 4 + (i & 1) * 2) * ROWS;
+            bool over = false;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const float2 sc = *reinterpret_cast<const float2 *>(sm_sc + n * 8 + 2 * t);
@@ -815,17 +835,41 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                     for (int c = 0; c < 4; c++)
                         if (key0 + 16 * half + (c >> 1) * 8 + (int)tok > ((c & 1) ? lim.y : lim.x)) s[n][c] = -INFINITY;
                 }
-                float x0 = fmaxf(s[n][0], s[n][2]), x1 = fmaxf(s[n][1], s[n][3]);
+                over |= fmaxf(s[n][0], s[n][2]) > R[n][0] + VF_LAG || fmaxf(s[n][1], s[n][3]) > R[n][1] + VF_LAG;
+            }
+            uint32_t move;
+            asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %2, 0;\n\tbarrier.cta.red.or.pred b, %1, 64, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+                         : "=r"(move) : "r"(1 + pair), "r"((uint32_t)over) : "memory");
+            if (move) {
+                float x[NT][2];
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                for (int n = 0; n < NT; n++) {
+                    x[n][0] = fmaxf(s[n][0], s[n][2]); x[n][1] = fmaxf(s[n][1], s[n][3]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        x[n][0] = fmaxf(x[n][0], __shfl_xor_sync(0xffffffffu, x[n][0], d));
+                        x[n][1] = fmaxf(x[n][1], __shfl_xor_sync(0xffffffffu, x[n][1], d));
+                    }
+                    if (g == 0) *reinterpret_cast<float2 *>(mx + half * ROWS + n * 8 + 2 * t) = make_float2(x[n][0], x[n][1]);
                 }
-                const float n0 = fmaxf(m[n][0], ceilf(x0)), n1 = fmaxf(m[n][1], ceilf(x1));
-                l[n][0] *= m[n][0] == n0 ? 1.0f : ex2(m[n][0] - n0);
-                l[n][1] *= m[n][1] == n1 ? 1.0f : ex2(m[n][1] - n1);
-                m[n][0] = n0; m[n][1] = n1;
-                const float b0 = (n0 == -INFINITY ? 0.0f : n0) - W_SHIFT, b1 = (n1 == -INFINITY ? 0.0f : n1) - W_SHIFT;
+                asm volatile("barrier.cta.sync %0, 64;" ::"r"(1 + pair) : "memory");
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float2 y = *reinterpret_cast<const float2 *>(mx + (half ^ 1) * ROWS + n * 8 + 2 * t);
+                    const float n0 = fmaxf(R[n][0], fmaxf(x[n][0], y.x)), n1 = fmaxf(R[n][1], fmaxf(x[n][1], y.y));
+                    const float f0 = R[n][0] == n0 ? 1.0f : ex2(R[n][0] - n0), f1 = R[n][1] == n1 ? 1.0f : ex2(R[n][1] - n1);
+                    l[n][0] *= f0; l[n][1] *= f1;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) { o[n][j][0] *= f0; o[n][j][1] *= f1; o[n][j][2] *= f0; o[n][j][3] *= f1; }
+                    R[n][0] = n0; R[n][1] = n1;
+                }
+            }
+
+            // ---- weights of this warp's keys, to the other warp as well ----
+            const float iv = pow2f(-ev);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float b0 = (R[n][0] == -INFINITY ? 0.0f : R[n][0]) - VF_SHIFT, b1 = (R[n][1] == -INFINITY ? 0.0f : R[n][1]) - VF_SHIFT;
                 uint32_t pb[2], pl[2];
                 float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
@@ -842,32 +886,13 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                 l[n][0] = fmaf(a0, iv, l[n][0]); l[n][1] = fmaf(a1, iv, l[n][1]);
                 if constexpr (F32) reinterpret_cast<uint4 *>(px + half * Cfg::PX)[n * 32 + lane] = make_uint4(pb[0], pb[1], pl[0], pl[1]);
                 else reinterpret_cast<uint2 *>(px + half * Cfg::PX)[n * 32 + lane] = make_uint2(pb[0], pb[1]);
-                if (g == 0) *reinterpret_cast<float2 *>(mx + half * ROWS + n * 8 + 2 * t) = make_float2(n0, n1);
             }
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory");
-
-            // ---- the running output to the common maximum ----
-            bool grow = false;
-            float nr[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const float2 a = *reinterpret_cast<const float2 *>(mx + n * 8 + 2 * t), b = *reinterpret_cast<const float2 *>(mx + ROWS + n * 8 + 2 * t);
-                nr[n][0] = fmaxf(a.x, b.x); nr[n][1] = fmaxf(a.y, b.y);
-                grow |= nr[n][0] > R[n][0] || nr[n][1] > R[n][1];
-            }
-            if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const float f0 = R[n][0] == nr[n][0] ? 1.0f : ex2(R[n][0] - nr[n][0]), f1 = R[n][1] == nr[n][1] ? 1.0f : ex2(R[n][1] - nr[n][1]);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) { o[n][j][0] *= f0; o[n][j][1] *= f1; o[n][j][2] *= f0; o[n][j][3] *= f1; }
-                    R[n][0] = nr[n][0]; R[n][1] = nr[n][1];
-                }
-            }
+            asm volatile("barrier.cta.sync %0, 64;" ::"r"(1 + pair) : "memory");
 
             // ---- O^T += V^T P^T: row g of tile j is dim 128 half + 16 g + 2 j, row g + 8 the dim after it ----
-            mbar_wait(&full[EV % NS], (EV / NS) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
-            uint8_t *vs = ring + (EV % NS) * 4096;
+            const uint32_t vsl = VS == 2 ? n_t & 1 : 0;
+            mbar_wait(&full_v[vsl], VS == 2 ? (n_t >> 1) & 1 : n_t & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
+            uint8_t *vs = ring + (2 + vsl) * 4096;
             if (key0 + TILE > n_keys) {                // rows past the last key may hold anything
                 for (int off = (n_keys - key0) * 128 + lane * 16; off < TILE * 128; off += 512) *reinterpret_cast<uint4 *>(vs + off) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
@@ -879,22 +904,12 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                 uint32_t b[NT][F32 ? 4 : 2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    // row g's weights times 2^(own maximum - common maximum), in two steps (fp16 ends at 2^-24)
-                    const float ma = mx[kk * ROWS + n * 8 + g], mb = mx[(kk ^ 1) * ROWS + n * 8 + g];
-                    const float d = ma >= mb ? 0.0f : fmaxf(ma - mb, -40.0f);
-                    const float d0 = fmaxf(d, -14.0f), d1 = fmaxf(d - d0, -24.0f);
-                    const __half2 f0 = __float2half2_rn(ex2(d0)), f1 = __float2half2_rn(ex2(d1));
                     if constexpr (F32) {
-                        const uint4 v = reinterpret_cast<const uint4 *>(px + kk * Cfg::PX)[n * 32 + lane];
-                        b[n][0] = v.x; b[n][1] = v.y; b[n][2] = v.z; b[n][3] = v.w;
+                        const uint4 x = reinterpret_cast<const uint4 *>(px + kk * Cfg::PX)[n * 32 + lane];
+                        b[n][0] = x.x; b[n][1] = x.y; b[n][2] = x.z; b[n][3] = x.w;
                     } else {
-                        const uint2 v = reinterpret_cast<const uint2 *>(px + kk * Cfg::PX)[n * 32 + lane];
-                        b[n][0] = v.x; b[n][1] = v.y;
-                    }
-#pragma unroll
-                    for (int c = 0; c < (F32 ? 4 : 2); c++) {
-                        const __half2 x = __hmul2(__hmul2(*reinterpret_cast<const __half2 *>(&b[n][c]), f0), f1);
-                        b[n][c] = *reinterpret_cast<const uint32_t *>(&x);
+                        const uint2 x = reinterpret_cast<const uint2 *>(px + kk * Cfg::PX)[n * 32 + lane];
+                        b[n][0] = x.x; b[n][1] = x.y;
                     }
                 }
                 const uint32_t ta = 16 * kk + 2 * t, tb = 16 * kk + ((2 * t + 1) ^ 4);
@@ -922,9 +937,9 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                 }
             }
             __syncwarp();
-            if (EV + NS < E1) load(EV + NS);
+            if (lane == 0 && i + AHEAD_V < nt) load_v(n_t + AHEAD_V, nv);
         }
-        E0 = E1;
+        done += nt;
 
         // ---- segment end: every warp puts its 128 dims of all rows into its slots, and all threads add them up ----
 #pragma unroll
@@ -933,7 +948,10 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
             for (int c = 0; c < 2; c++) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], d);
-                if (g == 0) { sm_m[warp * ROWS + n * 8 + 2 * t + c] = m[n][c]; sm_l[warp * ROWS + n * 8 + 2 * t + c] = l[n][c]; }
+                if (g == 0) {
+                    if (half == 0) sm_m[pair * ROWS + n * 8 + 2 * t + c] = R[n][c];
+                    sm_l[warp * ROWS + n * 8 + 2 * t + c] = l[n][c];
+                }
             }
         }
         if (nt > 0) {
@@ -950,31 +968,44 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                 }
         }
         __syncthreads();
+        if (threadIdx.x < ROWS) {                      // one thread per row: the maximum, the pairs' factors, the sum
+            const int row = threadIdx.x;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < PAIRS; k++) M = fmaxf(M, sm_m[k * ROWS + row]);
+#pragma unroll
+            for (int k = 0; k < PAIRS; k++) {
+                const float r = sm_m[k * ROWS + row], f = r == M ? 1.0f : ex2(r - M);
+                L = fmaf(sm_l[2 * k * ROWS + row] + sm_l[(2 * k + 1) * ROWS + row], f, L);
+                sm_m[k * ROWS + row] = f;
+            }
+            sm_t[row] = M; sm_t[ROWS + row] = L;
+        }
+        __syncthreads();
         const bool whole = seg_t0 == 0 && seg_n == sq.n_tiles;
         const size_t slot = (size_t)blockIdx.x + (size_t)w.s * p.kv_heads + w.h;
         const int in = min(PAIRS, seg_n);              // pairs that had a tile
         for (int idx = threadIdx.x; idx < valid * 64; idx += Cfg::THREADS) {
             const int row = idx >> 6, pc = idx & 63;
             const uint32_t piece = (uint32_t)(pc & 31) ^ (uint32_t)((row >> 1) & 3);
-            float M = -INFINITY;
-            for (int k = 0; k < 2 * in; k++) M = fmaxf(M, sm_m[k * ROWS + row]);
+            const float *src = reinterpret_cast<const float *>(smem + (pc >> 5) * NS * 4096) + row * 128 + piece * 4;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float L = 0.0f;
-            for (int k = 0; k < in; k++) {
-                const float ma = sm_m[2 * k * ROWS + row], mb = sm_m[(2 * k + 1) * ROWS + row], r = fmaxf(ma, mb);
-                const float f = r == M ? 1.0f : ex2(r - M);
-                L += sm_l[2 * k * ROWS + row] * (ma == M ? 1.0f : ex2(ma - M)) + sm_l[(2 * k + 1) * ROWS + row] * (mb == M ? 1.0f : ex2(mb - M));
-                const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + (2 * k + (pc >> 5)) * NS * 4096) + row * 128 + piece * 4);
-                acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y); acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+#pragma unroll
+            for (int k = 0; k < PAIRS; k++) {
+                if (k < in) {
+                    const float f = sm_m[k * ROWS + row];
+                    const float4 a = *reinterpret_cast<const float4 *>(src + (size_t)k * 2 * NS * 1024);
+                    acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y); acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+                }
             }
             if (whole) {
                 const int r = row / p.gqa;
-                const float inv = 1.0f / L;
+                const float inv = 1.0f / sm_t[ROWS + row];
                 store_out(p, sq, (size_t)r * p.q_heads + head0 + (row - r * p.gqa), pc * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
             } else {
                 const size_t pi = slot * p.slot_rows + row;
                 *reinterpret_cast<float4 *>(p.pacc + pi * 256 + pc * 4) = acc;
-                if (pc == 0) *reinterpret_cast<float2 *>(p.pstat + pi * 2) = make_float2(M, L);
+                if (pc == 0) *reinterpret_cast<float2 *>(p.pstat + pi * 2) = make_float2(sm_t[row], sm_t[ROWS + row]);
             }
         }
         T += seg_n;
