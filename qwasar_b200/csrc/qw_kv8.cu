@@ -305,7 +305,8 @@ constexpr int D_OFF_Q = D_WARPS * D_NS * ENTRY;
 constexpr int D_OFF_M = D_OFF_Q + 8192;                   // [warp][8]
 constexpr int D_OFF_L = D_OFF_M + D_WARPS * 32;
 constexpr int D_OFF_SC = D_OFF_L + D_WARPS * 32;          // [8]
-constexpr int D_OFF_BAR = D_OFF_SC + 32;                  // full[warps * slots], abort
+constexpr int D_OFF_T = D_OFF_SC + 32;                    // [2][8] maximum and sum of all warps
+constexpr int D_OFF_BAR = D_OFF_T + 64;                   // full[warps * slots], abort
 constexpr int D_SMEM = D_OFF_BAR + D_WARPS * D_NS * 8 + 16;
 static_assert(D_SMEM <= 232448, "exceeds the 227 KB a CTA may use");
 
@@ -318,27 +319,44 @@ __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
 }
 
-// One warp stages query row `row`: 8 dims per lane, scaled below 2^14 and put where the B fragments are read: step
-// 4 q + i takes dims 64 q + 16 t + 4 i + {0, 1 | 2, 3} of row g in lane (g, t).  `frag`: the row's tile of eight
-// (8 steps-pairs x 32 lanes x 16 bytes; f32: 16 steps, high and low parts).  sc: scale * log2(e) * the row's 2^qe.
+// Query row `row` of a group, 8 dims per lane, as it lies in memory.  A segment asks for its query rows BEFORE it asks for
+// keys and values: behind 200 KB of those per SM the rows came back 5 us later.
 template <bool F32>
-__device__ __forceinline__ void stage_q(const Kv8AttnParams &p, const Kv8AttnSeq &sq, int head0, int valid, int row, int lane, uint8_t *frags, float *sc) {
-    float x[8];
-#pragma unroll
-    for (int k = 0; k < 8; k++) x[k] = 0.0f;
+struct RowRaw { uint4 a, b; };
+template <bool F32>
+__device__ __forceinline__ RowRaw<F32> fetch_q(const Kv8AttnParams &p, const Kv8AttnSeq &sq, int head0, int valid, int row, int lane) {
+    RowRaw<F32> x;
+    x.a = x.b = make_uint4(0, 0, 0, 0);
     if (row < valid) {
         const int r = row / p.gqa, hh = row - r * p.gqa;
         const size_t at = ((size_t)r * p.q_heads + head0 + hh) * 256 + lane * 8;
-        if constexpr (F32) {
-            const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at);
-            const float4 b = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(sq.q) + at + 4);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __nv_bfloat16 *>(sq.q) + at);
-            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+        const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(sq.q) + at * (F32 ? 4 : 2));
+        x.a = src[0];
+        if (F32) x.b = src[1];
+    }
+    return x;
+}
+// Brings the query rows of the group a CTA turns to next (and a whole group's gate rows) into L2.
+__device__ __forceinline__ void prefetch_rows(const void *base, int io, size_t row0_el, size_t row_stride_el, int rows_of_call, int gqa, int q_heads, int i, int lane) {
+    if (i >= rows_of_call * gqa) return;
+    const int r = i / gqa, hh = i - r * gqa;
+    const size_t el = io == DT_F32 ? 4 : 2;
+    const uint8_t *at = reinterpret_cast<const uint8_t *>(base) + (row0_el + ((size_t)r * q_heads + hh) * row_stride_el) * el + lane * 8 * el;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+}
+// One warp stages a row: scaled below 2^14 and put where the B fragments are read: step 4 q + i takes dims
+// 64 q + 16 t + 4 i + {0, 1 | 2, 3} of row g in lane (g, t).  `frags`: per tile of eight rows 8 pairs of steps x 32 lanes x
+// 16 bytes (f32: 16 steps, high and low parts).  sc: scale * log2(e) * the row's 2^qe.
+template <bool F32>
+__device__ __forceinline__ void stage_q(const Kv8AttnParams &p, const RowRaw<F32> &raw, int row, int lane, uint8_t *frags, float *sc) {
+    float x[8];
+    if constexpr (F32) {
+        x[0] = __uint_as_float(raw.a.x); x[1] = __uint_as_float(raw.a.y); x[2] = __uint_as_float(raw.a.z); x[3] = __uint_as_float(raw.a.w);
+        x[4] = __uint_as_float(raw.b.x); x[5] = __uint_as_float(raw.b.y); x[6] = __uint_as_float(raw.b.z); x[7] = __uint_as_float(raw.b.w);
+    } else {
+        const uint32_t u[4] = {raw.a.x, raw.a.y, raw.a.z, raw.a.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
-        }
+        for (int k = 0; k < 4; k++) { x[2 * k] = __uint_as_float(u[k] << 16); x[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u); }
     }
     float mx = 0.0f;
 #pragma unroll
@@ -363,6 +381,18 @@ __device__ __forceinline__ void stage_q(const Kv8AttnParams &p, const Kv8AttnSeq
     }
 }
 
+// What this CTA reads later on and nothing hides: the gate rows of a group it finishes by itself, the query rows of the
+// group after it.  Row i of either.
+__device__ __forceinline__ void next_rows(const Kv8AttnParams &p, Where w, const Kv8AttnSeq &sq, int seg_t0, int seg_n, int T, int hi, int i, int lane) {
+    if (sq.gate && seg_t0 == 0 && seg_n == sq.n_tiles)
+        prefetch_rows(sq.gate, p.io, (size_t)w.h * p.gqa * p.gate_stride, p.gate_stride, sq.rows, p.gqa, p.q_heads, i, lane);
+    if (T + seg_n < hi) {
+        if (++w.h == p.kv_heads) { w.h = 0; w.s++; }
+        const Kv8AttnSeq &nx = p.seq[w.s];
+        prefetch_rows(nx.q, p.io, (size_t)w.h * p.gqa * 256, 256, nx.rows, p.gqa, p.q_heads, i, lane);
+    }
+}
+
 template <bool F32>
 __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_constant__ Kv8AttnParams p) {
     constexpr int KG = D_WARPS, NS = D_NS;
@@ -370,6 +400,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
     float *sm_m = reinterpret_cast<float *>(smem + D_OFF_M);
     float *sm_l = reinterpret_cast<float *>(smem + D_OFF_L);
     float *sm_sc = reinterpret_cast<float *>(smem + D_OFF_SC);
+    float *sm_t = reinterpret_cast<float *>(smem + D_OFF_T);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + D_OFF_BAR);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(full + KG * NS);
 
@@ -422,12 +453,15 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
                 win_e = (ek & 0xffff) | (ev << 16);
             }
         };
+        RowRaw<F32> raw;
+        if (warp < 8) raw = fetch_q<F32>(p, sq, head0, valid, warp, lane);
         if (nt > 0) {
             window(0);
             if (lane == 0) { load(sq, win_k, 0); load(sq, win_v, 1); }
         }
+        if (warp < 8) next_rows(p, w, sq, seg_t0, seg_n, T, hi, warp, lane);
 
-        if (warp < 8) stage_q<F32>(p, sq, head0, valid, warp, lane, smem + D_OFF_Q, sm_sc + warp);
+        if (warp < 8) stage_q<F32>(p, raw, warp, lane, smem + D_OFF_Q, sm_sc + warp);
         __syncthreads();
 
         float o[16][4];
@@ -594,22 +628,37 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
                 }
         }
         __syncthreads();
+        if (threadIdx.x < 8) {                         // one thread per row: the maximum, the warps' factors, the sum
+            const int row = threadIdx.x;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KG; k++) M = fmaxf(M, sm_m[k * 8 + row]);
+#pragma unroll
+            for (int k = 0; k < KG; k++) {
+                const float r = sm_m[k * 8 + row], f = r == M ? 1.0f : ex2(r - M);
+                L = fmaf(sm_l[k * 8 + row], f, L);
+                sm_m[k * 8 + row] = f;
+            }
+            sm_t[row] = M; sm_t[8 + row] = L;
+        }
+        __syncthreads();
         const bool whole = seg_t0 == 0 && seg_n == sq.n_tiles;
         const size_t slot = (size_t)blockIdx.x + (size_t)w.s * p.kv_heads + w.h;
         const int in = min(KG, seg_n);                 // warps that had a tile
         for (int idx = threadIdx.x; idx < valid * 64; idx += D_THREADS) {
             const int row = idx >> 6, pc = idx & 63;
             const uint32_t piece = (uint32_t)pc ^ (uint32_t)((row >> 1) & 3);
-            float M = -INFINITY;
-            for (int k = 0; k < in; k++) M = fmaxf(M, sm_m[k * 8 + row]);
+            const float *src = reinterpret_cast<const float *>(smem) + row * 256 + piece * 4;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float L = 0.0f;
-            for (int k = 0; k < in; k++) {
-                const float mk = sm_m[k * 8 + row], f = mk == M ? 1.0f : ex2(mk - M);
-                const float4 a = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem + k * NS * ENTRY) + row * 256 + piece * 4);
-                L = fmaf(sm_l[k * 8 + row], f, L);
-                acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y); acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+#pragma unroll
+            for (int k = 0; k < KG; k++) {
+                if (k < in) {
+                    const float f = sm_m[k * 8 + row];
+                    const float4 a = *reinterpret_cast<const float4 *>(src + k * (NS * ENTRY / 4));
+                    acc.x = fmaf(a.x, f, acc.x); acc.y = fmaf(a.y, f, acc.y); acc.z = fmaf(a.z, f, acc.z); acc.w = fmaf(a.w, f, acc.w);
+                }
             }
+            const float M = sm_t[row], L = sm_t[8 + row];
             if (whole) {
                 const int r = row / p.gqa;
                 const float inv = 1.0f / L;
@@ -736,6 +785,10 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
             tma_load_2d(dst, &p.maps[sq.vmap], 128 * half, row, &full_v[sl]);
             tma_load_2d(dst + 2048, &p.maps[sq.vmap], 128 * half, row + 16, &full_v[sl]);
         };
+        constexpr int PER = (ROWS + Cfg::WARPS - 1) / Cfg::WARPS;
+        RowRaw<F32> raw[PER];
+#pragma unroll
+        for (int u = 0; u < PER; u++) raw[u] = fetch_q<F32>(p, sq, head0, valid, warp + u * Cfg::WARPS, lane);
         if (nt > 0) {
             rows_from(0);
             const int k1 = __shfl_sync(0xffffffffu, win_k, 1), v1 = __shfl_sync(0xffffffffu, win_v, 1);
@@ -748,7 +801,12 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                 }
             }
         }
-        for (int row = warp; row < ROWS; row += Cfg::WARPS) stage_q<F32>(p, sq, head0, valid, row, lane, smem + Cfg::OFF_Q, sm_sc + row);
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int row = warp + u * Cfg::WARPS;
+            next_rows(p, w, sq, seg_t0, seg_n, T, hi, row, lane);
+            if (row < ROWS) stage_q<F32>(p, raw[u], row, lane, smem + Cfg::OFF_Q, sm_sc + row);
+        }
         if (threadIdx.x < ROWS) sm_lim[threadIdx.x] = (int)threadIdx.x < valid ? sq.base_pos + (int)threadIdx.x / p.gqa : n_keys - 1;
         __syncthreads();
 
