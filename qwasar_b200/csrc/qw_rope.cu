@@ -14,8 +14,8 @@ namespace qw {
 
 namespace {
 
-constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_ITEMS = 4 * ROPE_THREADS;      // vectors a block takes before the heads are split over more blocks
+constexpr int ROPE_THREADS = 128, FLY = 3;        // vectors (half layout: pairs of vectors) a thread has on their way at a time
+constexpr int ROPE_ITEMS = FLY * ROPE_THREADS;    // what a block takes at once: beyond that the heads are split over more blocks
 
 template <typename T> struct Vec;                 // 16 bytes of T
 template <> struct Vec<float> {
@@ -59,8 +59,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeParams p, 
     const int per_rot = (INTER && VEC) ? N / 2 : N;
     const int n_rot = half / per_rot, n_cp = copy ? (p.head_dim - p.rotary_dim) / N : 0;
     const int per = n_rot + n_cp, total = nh * per;
-    // FLY vectors (half layout: pairs of vectors) of a thread are on their way at a time, the first ones under the angles
-    constexpr int FLY = 4;
+    // (the first vectors are asked for in front of the angles)
     uint4 a[FLY], b[FLY];
     int off[FLY], idx[FLY];
     auto fetch = [&](int it0) {
