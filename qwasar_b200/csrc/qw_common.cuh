@@ -13,7 +13,7 @@
 #define QW_KV8_BLOCK 64          // tokens of one head that share an exponent in an 8-bit cache
 #define QW_KV8_E_MIN (-60)       // exponents of an 8-bit cache are kept in this range (a block of zeros has the lowest)
 #define QW_KV8_E_MAX 119
-#define QW_KV8_MAPS 32           // the same for 8-bit caches
+#define QW_KV8_MAPS 16           // the same for 8-bit caches
 #define QW_MAX_MAPS 8            // distinct cache tensor maps one launch carries (arenas of one pool share theirs)
 
 // Status codes a kernel leaves in the backend's status word (first one wins).

@@ -258,7 +258,8 @@ struct Kv8AttnSeq {
     const void *q;           // [rows, q_heads, 256]
     void *out;
     const void *gate;        // nullptr, or element (r, h, d) at gate[(r*q_heads + h)*gate_stride + d]
-    Kv8Layer kc, vc;
+    const int32_t *ktab, *vtab;      // page tables [kv_heads, pt_stride]; nullptr: linear
+    const uint8_t *kexp, *vexp;      // exponent bytes [kv_heads, exp_stride]
     int32_t rows, base_pos;  // row r reads keys [0, base_pos + r]
     int32_t n_tiles;         // 32-key tiles per kv head
     int32_t cum_tiles;       // tiles of all earlier sequences times kv_heads
@@ -268,6 +269,7 @@ struct Kv8AttnParams {
     CUtensorMap maps[QW_KV8_MAPS];     // code rows, boxes of 128 bytes x kv8_box_rows() rows, SWIZZLE_128B
     Kv8AttnSeq seq[QW_MAX_SEQ];
     int32_t n_seq, q_heads, kv_heads, gqa;
+    int32_t pt_stride, max_ctx, exp_stride;      // the caches of one call have one shape
     int32_t total_tiles, n_cta, slot_rows;
     int32_t share[257];      // CTA c takes tiles [share[c], share[c + 1]) of the line
     int32_t io, gate_stride;

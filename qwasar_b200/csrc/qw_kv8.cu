@@ -62,6 +62,14 @@ __device__ __forceinline__ int64_t code_row(const Kv8Layer &L, int h, int t) {
     return pg < 0 ? -1 : (int64_t)pg * QW_KV8_PAGE_TOKENS + (t & (QW_KV8_PAGE_TOKENS - 1));
 }
 
+// The same from a launch's fields (attention: one head of one sequence).
+__device__ __forceinline__ int tile_row(const Kv8AttnParams &p, const int32_t *table, int h, int t) {
+    if (!table) return h * p.max_ctx + t;
+    const int pg = __ldg(table + (size_t)h * p.pt_stride + t / QW_KV8_PAGE_TOKENS);
+    if (pg < 0) report(p.status, QW_ST_BAD_PAGE);
+    return max(pg, 0) * QW_KV8_PAGE_TOKENS + (t & (QW_KV8_PAGE_TOKENS - 1));
+}
+
 // =======================================================================================
 // append
 // =======================================================================================
@@ -446,11 +454,9 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
             const int i = i0 + lane;
             if (i < nt) {
                 const int key = (seg_t0 + warp + i * KG) * TILE;
-                const int64_t kr = code_row(sq.kc, w.h, key), vr = code_row(sq.vc, w.h, key);
-                if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
-                win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
-                const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + key / BLK]);
-                const int ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + key / BLK]);
+                win_k = tile_row(p, sq.ktab, w.h, key); win_v = tile_row(p, sq.vtab, w.h, key);
+                const int ek = clamp_exp(sq.kexp[(size_t)w.h * p.exp_stride + key / BLK]);
+                const int ev = clamp_exp(sq.vexp[(size_t)w.h * p.exp_stride + key / BLK]);
                 win_e = (ek & 0xffff) | (ev << 16);
             }
         };
@@ -704,7 +710,7 @@ struct VfCfg {
     static constexpr int OFF_T = OFF_L + WARPS * ROWS * 4;      // [2][ROWS] maximum and sum of all pairs
     static constexpr int OFF_SC = OFF_T + 2 * ROWS * 4;         // [ROWS]
     static constexpr int OFF_LIM = OFF_SC + ROWS * 4;           // [ROWS] last key of a row
-    static constexpr int OFF_BAR = OFF_LIM + ROWS * 4;          // full[warp][slot], abort
+    static constexpr int OFF_BAR = OFF_LIM + ROWS * 4;           // full[warp][slot], abort
     static constexpr int SMEM = OFF_BAR + WARPS * NS * 8 + 16;
     static_assert(SMEM <= 232448, "exceeds the 227 KB a CTA may use");
     static_assert(NT <= NS, "a warp's sums do not fit its slots");
@@ -761,14 +767,12 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
         auto key_of = [&](int i) { return (seg_t0 + pair + i * PAIRS) * TILE; };
         auto rows_from = [&](int i0) {
             if (i0 + lane >= nt) return;
-            const int64_t kr = code_row(sq.kc, w.h, key_of(i0 + lane)), vr = code_row(sq.vc, w.h, key_of(i0 + lane));
-            if (kr < 0 || vr < 0) report(p.status, QW_ST_BAD_PAGE);
-            win_k = (int)(kr < 0 ? 0 : kr); win_v = (int)(vr < 0 ? 0 : vr);
+            win_k = tile_row(p, sq.ktab, w.h, key_of(i0 + lane)); win_v = tile_row(p, sq.vtab, w.h, key_of(i0 + lane));
         };
         auto exps_from = [&](int i0) {
             if (i0 + lane >= nt) return;
             const int b = key_of(i0 + lane) / BLK;
-            const int ek = clamp_exp(sq.kc.exps[(size_t)w.h * sq.kc.exp_stride + b]), ev = clamp_exp(sq.vc.exps[(size_t)w.h * sq.vc.exp_stride + b]);
+            const int ek = clamp_exp(sq.kexp[(size_t)w.h * p.exp_stride + b]), ev = clamp_exp(sq.vexp[(size_t)w.h * p.exp_stride + b]);
             win_e = (ek & 0xffff) | (ev << 16);
         };
         // lane 0: this warp's 16 keys x 256 dims of K, and 32 keys x 128 dims of V, of the pair's n-th tile
@@ -1077,7 +1081,9 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
         for (int i = 0; i < 4096; i++) __nanosleep(10000);
 }
 
-// Partials of a cut group: one block per (group, row).  Slices of 64 threads x four dims take every MG_SLICES-th
+// Partials of a cut group: one block per (group, row).  (A kernel of its own: it starts under the attention kernel's tail,
+// and the next call's attention under its own.  Added up by the last CTA of a group instead, behind a counter, a decode
+// step over 4 K keys took 12.2 us against 8.9.)  Slices of 64 threads x four dims take every MG_SLICES-th
 // partial each, ten loads in flight, asked for before the weights are known: one trip to L2 for up to 40 partials
 // (four slices: many groups, few partials each) or 160 (sixteen: few groups, cut over most of the SMs).
 constexpr int MG_FLY = 10;
@@ -1236,19 +1242,32 @@ void kv8_attn_plan(Kv8AttnParams &p) {
     // line is cut evenly, and a cut among the virtual tiles moves to the group's first real one.
     const int groups = p.n_seq * p.kv_heads;
     const int64_t v_total = (int64_t)cum + (int64_t)SEG_COST * groups;
-    int s = 0, h = 0;
-    int64_t v0 = 0;                                          // virtual start of group (s, h)
-    int t0 = 0;                                              // its first real tile
+    int s = 0, h = 0, t0 = 0;                                // group (s, h) and its first real tile
+    int64_t v0 = 0, v = 0, rest = 0;                         // its virtual start; v = floor(v_total * c / n_cta)
+    const int64_t step = v_total / p.n_cta, more = v_total % p.n_cta;
     for (int c = 0; c < p.n_cta; c++) {
-        const int64_t v = v_total * c / p.n_cta;
         while (v >= v0 + SEG_COST + p.seq[s].n_tiles) {
             v0 += SEG_COST + p.seq[s].n_tiles;
             t0 += p.seq[s].n_tiles;
             if (++h == p.kv_heads) { h = 0; s++; }
         }
         p.share[c] = t0 + (int)std::max<int64_t>(0, v - v0 - SEG_COST);
+        v += step;
+        rest += more;
+        if (rest >= p.n_cta) { rest -= p.n_cta; v++; }
     }
     p.share[p.n_cta] = cum;
+}
+
+// Partials of the group that has the most (0: no group is cut).
+static int most_parts(const Kv8AttnParams &p) {
+    int parts = 0;
+    for (int i = 0; i < p.n_seq; i++)
+        for (int h = 0; h < p.kv_heads; h++) {
+            const int g0 = p.seq[i].cum_tiles + h * p.seq[i].n_tiles;
+            parts = std::max(parts, share_of(p, g0 + p.seq[i].n_tiles - 1) - share_of(p, g0));
+        }
+    return parts ? parts + 1 : 0;
 }
 
 size_t kv8_attn_scratch_bytes(const Kv8AttnParams &p) {
@@ -1265,13 +1284,7 @@ void launch_kv8_attn(cudaStream_t s, Kv8AttnParams &p, int max_rows, void *scrat
     else if (nt == 2) { if (f32) launch_verify_t<2, true>(s, p); else launch_verify_t<2, false>(s, p); }
     else if (nt == 3) { if (f32) launch_verify_t<3, true>(s, p); else launch_verify_t<3, false>(s, p); }
     else { if (f32) launch_verify_t<4, true>(s, p); else launch_verify_t<4, false>(s, p); }
-    int parts = 0;                             // most partials of a cut group
-    for (int i = 0; i < p.n_seq; i++)
-        for (int h = 0; h < p.kv_heads; h++) {
-            const int g0 = p.seq[i].cum_tiles + h * p.seq[i].n_tiles;
-            parts = std::max(parts, share_of(p, g0 + p.seq[i].n_tiles - 1) - share_of(p, g0));
-        }
-    if (parts) parts++;
+    const int parts = most_parts(p);
     if (!parts) return;                        // every group was written whole
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;

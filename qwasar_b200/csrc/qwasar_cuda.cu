@@ -2165,6 +2165,7 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
     Kv8AttnParams p;
     memset(&p, 0, sizeof p);
     p.q_heads = q_heads; p.kv_heads = kv_heads; p.gqa = gqa; p.io = io; p.gate_stride = gate_stride; p.scale = scale;
+    p.max_ctx = max_ctx; p.exp_stride = (int32_t)kv8_blocks(max_ctx);
     int n_maps = 0, max_rows = 0;
     int64_t tiles = 0;
     auto flush = [&]() {
@@ -2217,7 +2218,9 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
             s.q = qp + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
             s.out = op + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
             s.gate = gp ? gp + (size_t)r0 * q_heads * gate_stride * el : nullptr;
-            s.kc = kc; s.vc = vc; s.rows = rr; s.base_pos = a.base_pos + r0;
+            s.ktab = kc.table; s.vtab = vc.table; s.kexp = kc.exps; s.vexp = vc.exps;
+            s.rows = rr; s.base_pos = a.base_pos + r0;
+            if (kc.table) p.pt_stride = kc.pt_stride;
             s.kmap = (uint8_t)ks; s.vmap = (uint8_t)vs;
             max_rows = std::max(max_rows, rr);
             tiles += add;
