@@ -301,7 +301,7 @@ struct Kv8PrefillParams {
     float *pacc, *pstat;     // splits > 1: per (tile, kv head, share) sums and (max, sum) per tile row
     int *status;
 };
-int kv8_prefill_splits(int tiles, int steps, int sms);
+int kv8_prefill_splits(int tiles, int steps, int sms, double *us = nullptr);
 size_t kv8_prefill_scratch_bytes(const Kv8PrefillParams &p);
 void launch_kv8_prefill(cudaStream_t s, Kv8PrefillParams &p, void *scratch);
 

@@ -493,9 +493,13 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
             const int nk = __shfl_sync(0xffffffffu, win_k, (i + 1) & 31), nv = __shfl_sync(0xffffffffu, win_v, (i + 1) & 31);
 
             // ---- S^T = K Q^T ----
-            float s[2][4];
+            // (f32: the tensor op's running sum loses a little at every step, so the high parts of even and odd steps and
+            // the low parts have sums of their own)
+            float s[2][4], s1[2][4], sl[2][4];
 #pragma unroll
-            for (int n = 0; n < 2; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[n][c] = s1[n][c] = sl[n][c] = 0.0f;
             mbar_wait(&full[0], phase, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
 #pragma unroll
             for (int q = 0; q < 4; q++) {
@@ -514,8 +518,8 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
                         for (int n = 0; n < 2; n++) {
                             const uint32_t a0 = f16x2_lo(kw[2 * n][k]), a1 = f16x2_lo(kw[2 * n + 1][k]), a2 = f16x2_hi(kw[2 * n][k]), a3 = f16x2_hi(kw[2 * n + 1][k]);
                             if constexpr (F32) {
-                                mma_f16(s[n], a0, a1, a2, a3, qf[h][0], qf[h][1]);
-                                mma_f16(s[n], a0, a1, a2, a3, qf[h][2], qf[h][3]);
+                                mma_f16(h ? s1[n] : s[n], a0, a1, a2, a3, qf[h][0], qf[h][1]);
+                                mma_f16(sl[n], a0, a1, a2, a3, qf[h][2], qf[h][3]);
                             } else {
                                 mma_f16(s[n], a0, a1, a2, a3, qf[0][2 * h], qf[0][2 * h + 1]);
                             }
@@ -527,6 +531,12 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
             if (lane == 0 && i + 1 < nt) load(sq, nk, 0);
 
             // ---- online softmax ----
+            if constexpr (F32) {
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s[n][c] += s1[n][c] + sl[n][c];
+            }
             const float k0 = sc0 * pow2f(ek), k1 = sc1 * pow2f(ek), fv = (float)ev;
 #pragma unroll
             for (int n = 0; n < 2; n++)
@@ -841,9 +851,11 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
             const int ek = (int)(int16_t)(ex & 0xffff), ev = ex >> 16;
 
             // ---- S^T = K Q^T for this warp's 16 keys ----
-            float s[NT][4];
+            float s[NT][4], sl[NT][4];                 // (f32: the low parts have sums of their own, as in the decode kernel)
 #pragma unroll
-            for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[n][c] = sl[n][c] = 0.0f;
             mbar_wait(&full_k[n_t & 1], (n_t >> 1) & 1, abort_flag, p.status, QW_ST_TMA_TIMEOUT);
             {
                 const uint32_t kb = smem_u32(ring + (n_t & 1) * 4096) + tok * 128;
@@ -871,7 +883,7 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
                             for (int n = 0; n < NT; n++) {
                                 if constexpr (F32) {
                                     mma_f16(s[n], a0, a1, a2, a3, b[n][0], b[n][1]);
-                                    mma_f16(s[n], a0, a1, a2, a3, b[n][2], b[n][3]);
+                                    mma_f16(sl[n], a0, a1, a2, a3, b[n][2], b[n][3]);
                                 } else {
                                     mma_f16(s[n], a0, a1, a2, a3, b[n][2 * h], b[n][2 * h + 1]);
                                 }
@@ -891,7 +903,7 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
             for (int n = 0; n < NT; n++) {
                 const float2 sc = *reinterpret_cast<const float2 *>(sm_sc + n * 8 + 2 * t);
 #pragma unroll
-                for (int c = 0; c < 4; c++) s[n][c] = fmaf(s[n][c], ((c & 1) ? sc.y : sc.x) * fk, fv);
+                for (int c = 0; c < 4; c++) s[n][c] = fmaf(F32 ? s[n][c] + sl[n][c] : s[n][c], ((c & 1) ? sc.y : sc.x) * fk, fv);
                 if (masked) {
                     const int2 lim = *reinterpret_cast<const int2 *>(sm_lim + n * 8 + 2 * t);
 #pragma unroll

@@ -670,19 +670,21 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
 
 }  // namespace
 
-// How the keys of every tile are cut.  A step of 128 keys takes about 1.4 us, what a CTA does outside its steps about
-// 6 us; CTAs run one per SM, so the launch takes the number of rounds times the length of a share, and a cut launch
-// writes and reads 128 KB of sums per share on top.
-int kv8_prefill_splits(int tiles, int steps, int sms) {
+// How the keys of every tile are cut, and about how long the launch takes.  A step of 128 keys takes about 1.6 us, what a CTA
+// does outside its steps about 9.5 us; CTAs run one per SM, so the launch takes the number of rounds times the length of a
+// share, and a cut launch writes and reads up to 128 KB of sums per share on top.
+// (4 kv heads: 48 query rows behind 4096 keys 15.0 us, the rule says 15.2; 499 tokens of 24 heads behind 16 K 176 and 169.)
+int kv8_prefill_splits(int tiles, int steps, int sms, double *us) {
     int best = 1;
     double best_us = 0.0;
     for (int s = 1; s <= std::min(steps, 64); s++) {
         const int64_t ctas = (int64_t)tiles * s;
         if (s > 1 && ctas > 4 * sms) break;
         const double rounds = (double)((ctas + sms - 1) / sms);
-        const double us = rounds * (1.4 * ((steps + s - 1) / s) + 6.0) + (s > 1 ? 4.0 + ctas * 0.05 : 0.0);
-        if (s == 1 || us < best_us) { best = s; best_us = us; }
+        const double t = rounds * (1.6 * ((steps + s - 1) / s) + 9.5) + (s > 1 ? 0.5 + ctas * 0.03 : 0.0);
+        if (s == 1 || t < best_us) { best = s; best_us = t; }
     }
+    if (us) *us = best_us;
     return best;
 }
 size_t kv8_prefill_scratch_bytes(const Kv8PrefillParams &p) {

@@ -2160,8 +2160,23 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
     const size_t n = (size_t)rows * q_heads, bytes = n * QW_HEAD_DIM * el;
     const int chunk = std::max(1, most / gqa);
     const uint32_t box = kv8_box_rows(std::min(rows, chunk) * gqa);
-    // many bf16 rows on the tcgen05 kernel (which needs a scale it can multiply masked scores by)
-    const bool tiled = rows * gqa > most && io == QW_BF16 && fabsf(scale) > 1e-12f && fabsf(scale) < 1e12f;
+    // More query rows than the split kernels take at once: bf16 on the tcgen05 kernel, one launch per sequence, or in chunks
+    // of the split kernels, one launch for all of them but every chunk reads its keys again.  By what the two take
+    // (measured, one sequence of 4 kv heads: 48 query rows over 256 keys 16.6 us against 11.9, over 1024 12.8 against 11.7,
+    // over 16 K 23 against 38; 192 over 4 K 18 against 37; five sequences of 32 over 4 K 74 against 43): a launch of the split kernels about 11 us and 3.2 TB/s of keys and values.  (The tcgen05
+    // kernel also needs a scale that it can multiply a masked score by.)
+    bool tiled = false;
+    if (rows * gqa > most && io == QW_BF16 && fabsf(scale) > 1e-12f && fabsf(scale) < 1e12f) {
+        const int tile_rows = 128 / gqa, tiles = (rows + tile_rows - 1) / tile_rows * kv_heads, chunks = (rows + chunk - 1) / chunk;
+        double tc_us = 0.0, split_us = 11.0;
+        for (int i = 0; i < n_seq; i++) {
+            double us;
+            kv8_prefill_splits(tiles, (calls[i].base_pos + (rows + 1) / 2 + 127) / 128, sm_count(), &us);
+            tc_us += us;
+            split_us += (double)chunks * kv_heads * (calls[i].base_pos + rows / 2) * (2.0 * QW_HEAD_DIM) / 3.2e6;
+        }
+        tiled = tc_us <= split_us;
+    }
     Kv8AttnParams p;
     memset(&p, 0, sizeof p);
     p.q_heads = q_heads; p.kv_heads = kv_heads; p.gqa = gqa; p.io = io; p.gate_stride = gate_stride; p.scale = scale;
