@@ -71,13 +71,13 @@ __device__ __forceinline__ uint32_t e4m3x2_of_f16(uint32_t v) {
     return r;
 }
 // a * sigmoid(g), b * sigmoid(h): two exponentials and one reciprocal (the unit that works them out delivers 16 a clock,
-// and the output tile has 32 768 elements).  Gates below -43 count as -43: 2e-19.
+// and the output tile has 32 768 elements).  Gates below -43 count as -43: 2e-19.  A NaN stays in its own element.
 __device__ __forceinline__ void gate2(float &a, float &b, float g, float h) {
     const float u = 1.0f + __expf(-fmaxf(g, -43.0f)), v = 1.0f + __expf(-fmaxf(h, -43.0f));
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * v));
-    a *= r * v;
-    b *= r * u;
+    a = g == g ? a * (r * v) : g;
+    b = h == h ? b * (r * u) : h;
 }
 __device__ __forceinline__ uint32_t f16x2_of(uint32_t codes16) {
     uint32_t r;

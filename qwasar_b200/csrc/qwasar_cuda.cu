@@ -2086,19 +2086,23 @@ bool kv8_write(qw_cmd c, int n_seq, const qw_ref *kcache, const qw_ref *vcache, 
     }
     if (rows == 0) return true;
     const size_t bytes = ((size_t)(rows - 1) * row_stride + width) * el;
+    std::vector<Kv8WriteSeq> seqs((size_t)n_seq);            // (all of them before the first launch: a refused call encodes nothing)
+    for (int i = 0; i < n_seq; i++) {
+        Kv8WriteSeq &q = seqs[i];
+        q.base_pos = base_pos[i];
+        q.k = near_range(c, k[i], bytes, false);
+        q.v = near_range(c, v[i], bytes, false);
+        if (!q.k || !q.v) return false;
+        if (!resolve_kv8(c, kcache[i], kv_heads, max_ctx, q.base_pos, q.base_pos + rows, true, &q.kc, nullptr) ||
+            !resolve_kv8(c, vcache[i], kv_heads, max_ctx, q.base_pos, q.base_pos + rows, true, &q.vc, nullptr)) return false;
+    }
     for (int s0 = 0; s0 < n_seq; s0 += QW_MAX_SEQ) {
         Kv8WriteParams p;
         memset(&p, 0, sizeof p);
         p.n_seq = std::min(QW_MAX_SEQ, n_seq - s0);
         for (int i = 0; i < p.n_seq; i++) {
-            Kv8WriteSeq &q = p.seq[i];
-            const int32_t b = base_pos[s0 + i];
-            q.base_pos = b;
-            q.k = near_range(c, k[s0 + i], bytes, false);
-            q.v = near_range(c, v[s0 + i], bytes, false);
-            if (!q.k || !q.v) return false;
-            if (!resolve_kv8(c, kcache[s0 + i], kv_heads, max_ctx, b, b + rows, true, &q.kc, nullptr) ||
-                !resolve_kv8(c, vcache[s0 + i], kv_heads, max_ctx, b, b + rows, true, &q.vc, nullptr)) return false;
+            p.seq[i] = seqs[s0 + i];
+            const int32_t b = p.seq[i].base_pos;
             p.max_blocks = std::max(p.max_blocks, (b + rows - 1) / QW_KV8_BLOCK - b / QW_KV8_BLOCK + 1);
         }
         p.row_stride = row_stride; p.rows = rows; p.kv_heads = kv_heads; p.io = io;
@@ -2113,14 +2117,22 @@ struct Kv8Call {
     qw_ref out, gate, q, kcache, vcache;
     int32_t base_pos;
 };
+// Its operands, looked up.
+struct Kv8Ready {
+    const char *q, *gate;
+    char *out;
+    Kv8Layer kc, vc;
+    CUtensorMap km, vm;
+    bool tiled;                                              // on the tcgen05 kernel
+};
 
 // Many bf16 rows: the tcgen05 kernel.
-bool kv8_prefill(qw_cmd c, const Kv8Call &a, const void *q, void *out, const void *gate, int32_t rows, int32_t q_heads, int32_t kv_heads,
-                 int32_t max_ctx, float scale, int32_t gate_stride) {
+bool kv8_prefill(qw_cmd c, const Kv8Ready &a, int32_t base_pos, int32_t rows, int32_t q_heads, int32_t kv_heads, float scale, int32_t gate_stride) {
+    const char *q = a.q, *gate = a.gate;
+    char *out = a.out;
     Kv8PrefillParams p;
     memset(&p, 0, sizeof p);
-    const int32_t end = a.base_pos + rows;
-    if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &p.kc, &p.kmap, 64) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &p.vc, nullptr)) return false;
+    p.kc = a.kc; p.vc = a.vc; p.kmap = a.km;
     p.gqa = q_heads / kv_heads;
     p.tile_rows = 128 / p.gqa;
     if (!encode_heads_map(&p.qmap, q, rows, q_heads, QW_HEAD_DIM, p.gqa, p.tile_rows) || !encode_heads_map(&p.omap, out, rows, q_heads, QW_HEAD_DIM, p.gqa, p.tile_rows) ||
@@ -2129,10 +2141,10 @@ bool kv8_prefill(qw_cmd c, const Kv8Call &a, const void *q, void *out, const voi
     p.out = reinterpret_cast<__nv_bfloat16 *>(out);
     p.gate = reinterpret_cast<const __nv_bfloat16 *>(gate);
     p.gate_stride = gate_stride; p.gated = gate != nullptr;
-    p.rows = rows; p.base_pos = a.base_pos; p.q_heads = q_heads; p.kv_heads = kv_heads;
+    p.rows = rows; p.base_pos = base_pos; p.q_heads = q_heads; p.kv_heads = kv_heads;
     p.n_q_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
     p.box_bytes = 128 * p.gqa * p.tile_rows;
-    p.splits = kv8_prefill_splits(p.n_q_tiles * kv_heads, (a.base_pos + (rows + 1) / 2 + 127) / 128, sm_count());
+    p.splits = kv8_prefill_splits(p.n_q_tiles * kv_heads, (base_pos + (rows + 1) / 2 + 127) / 128, sm_count());
     p.scale = scale;
     p.status = cmd_status(c);
     void *scr = nullptr;
@@ -2163,8 +2175,8 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
     // More query rows than the split kernels take at once: bf16 on the tcgen05 kernel, one launch per sequence, or in chunks
     // of the split kernels, one launch for all of them but every chunk reads its keys again.  By what the two take
     // (measured, one sequence of 4 kv heads: 48 query rows over 256 keys 16.6 us against 11.9, over 1024 12.8 against 11.7,
-    // over 16 K 23 against 38; 192 over 4 K 18 against 37; five sequences of 32 over 4 K 74 against 43): a launch of the split kernels about 11 us and 3.2 TB/s of keys and values.  (The tcgen05
-    // kernel also needs a scale that it can multiply a masked score by.)
+    // over 16 K 23 against 38; 192 over 4 K 18 against 37; five sequences of 48 over 4 K 74 against 43): a launch of the split kernels about 11 us and
+    // 3.2 TB/s of keys and values.  (The tcgen05 kernel also needs a scale that it can multiply a masked score by.)
     bool tiled = false;
     if (rows * gqa > most && io == QW_BF16 && fabsf(scale) > 1e-12f && fabsf(scale) < 1e12f) {
         const int tile_rows = 128 / gqa, tiles = (rows + tile_rows - 1) / tile_rows * kv_heads, chunks = (rows + chunk - 1) / chunk;
@@ -2176,6 +2188,19 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
             split_us += (double)chunks * kv_heads * (calls[i].base_pos + rows / 2) * (2.0 * QW_HEAD_DIM) / 3.2e6;
         }
         tiled = tc_us <= split_us;
+    }
+    std::vector<Kv8Ready> ready((size_t)n_seq);              // (all of them before the first launch: a refused call encodes nothing)
+    for (int i = 0; i < n_seq; i++) {
+        const Kv8Call &a = calls[i];
+        Kv8Ready &r = ready[i];
+        const int32_t end = a.base_pos + rows;
+        r.q = (const char *)near_range(c, a.q, bytes, false);
+        r.out = (char *)near_range(c, a.out, bytes, true);
+        r.gate = a.gate.buf ? (const char *)near_range(c, a.gate, ((n - 1) * gate_stride + QW_HEAD_DIM) * el, false) : nullptr;
+        if (!r.q || !r.out || (a.gate.buf && !r.gate)) return false;
+        r.tiled = tiled && attn_prefill_io_ok(r.out, DT_BF16, r.gate, DT_BF16, gate_stride);
+        if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &r.kc, &r.km, r.tiled ? 64 : box) ||
+            !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &r.vc, r.tiled ? nullptr : &r.vm, box)) return false;
     }
     Kv8AttnParams p;
     memset(&p, 0, sizeof p);
@@ -2201,41 +2226,34 @@ bool attn_kv8(qw_cmd c, const Kv8Call *calls, int n_seq, int32_t rows, int32_t q
         return n_maps++;
     };
     for (int i = 0; i < n_seq; i++) {
-        const Kv8Call &a = calls[i];
-        Kv8Layer kc, vc;
-        CUtensorMap km, vm;
-        const int32_t end = a.base_pos + rows;
-        if (!resolve_kv8(c, a.kcache, kv_heads, max_ctx, 0, end, false, &kc, &km, box) || !resolve_kv8(c, a.vcache, kv_heads, max_ctx, 0, end, false, &vc, &vm, box)) return false;
-        const char *qp = (const char *)near_range(c, a.q, bytes, false);
-        char *op = (char *)near_range(c, a.out, bytes, true);
-        const char *gp = a.gate.buf ? (const char *)near_range(c, a.gate, ((n - 1) * gate_stride + QW_HEAD_DIM) * el, false) : nullptr;
-        if (!qp || !op || (a.gate.buf && !gp)) return false;
-        if (tiled && attn_prefill_io_ok(op, DT_BF16, gp, DT_BF16, gate_stride)) {
-            if (!flush()) return false;
-            if (!kv8_prefill(c, a, qp, op, gp, rows, q_heads, kv_heads, max_ctx, scale, gate_stride)) return false;
+        const Kv8Ready &a = ready[i];
+        const int32_t base_pos = calls[i].base_pos;
+        if (a.tiled) {
+            if (!flush() || !kv8_prefill(c, a, base_pos, rows, q_heads, kv_heads, scale, gate_stride)) return false;
             continue;
         }
         for (int r0 = 0; r0 < rows; r0 += chunk) {
             const int rr = std::min(chunk, rows - r0);
-            const int64_t add = (int64_t)((a.base_pos + r0 + rr + 31) / 32) * kv_heads;
+            const int64_t add = (int64_t)((base_pos + r0 + rr + 31) / 32) * kv_heads;
             int ks = -1, vs = -1;
             for (int attempt = 0; attempt < 2 && vs < 0; attempt++) {
                 if (attempt && !flush()) return false;
                 if (p.n_seq == QW_MAX_SEQ || tiles + add > 0x3fffffff) continue;
                 const int saved = n_maps;
-                ks = map_slot(km);
-                vs = ks < 0 ? -1 : map_slot(vm);
+                ks = map_slot(a.km);
+                vs = ks < 0 ? -1 : map_slot(a.vm);
                 if (vs < 0) n_maps = saved;
             }
             if (vs < 0) { cmd_fail(c, "attn_kv8: the call does not fit a launch"); return false; }
             Kv8AttnSeq &s = p.seq[p.n_seq++];
             memset(&s, 0, sizeof s);
-            s.q = qp + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
-            s.out = op + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
-            s.gate = gp ? gp + (size_t)r0 * q_heads * gate_stride * el : nullptr;
-            s.ktab = kc.table; s.vtab = vc.table; s.kexp = kc.exps; s.vexp = vc.exps;
-            s.rows = rr; s.base_pos = a.base_pos + r0;
-            if (kc.table) p.pt_stride = kc.pt_stride;
+            s.q = a.q + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
+            s.out = a.out + (size_t)r0 * q_heads * QW_HEAD_DIM * el;
+            s.gate = a.gate ? a.gate + (size_t)r0 * q_heads * gate_stride * el : nullptr;
+            s.ktab = a.kc.table; s.vtab = a.vc.table; s.kexp = a.kc.exps; s.vexp = a.vc.exps;
+            s.rows = rr; s.base_pos = base_pos + r0;
+            if (a.kc.table) p.pt_stride = a.kc.pt_stride;
+            if (a.vc.table) p.pt_stride = a.vc.pt_stride;
             s.kmap = (uint8_t)ks; s.vmap = (uint8_t)vs;
             max_rows = std::max(max_rows, rr);
             tiles += add;

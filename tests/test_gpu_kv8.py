@@ -361,6 +361,165 @@ def test_attn_batch(be, io, rows):
         B.all = [pool]
 
 
+@pytest.mark.parametrize("rows,base,qh,heads", [(300, 700, 9, 3), (400, 300, 15, 3), (600, 40, 32, 1), (1200, 0, 24, 4), (170, 2300, 21, 3)])
+def test_attn_many_rows_of_odd_groupings(be, rows, base, qh, heads):
+    """Groupings that do not divide a tile of 128 query rows, one and several shares of the keys."""
+    rng = np.random.default_rng(rows + qh)
+    got, want = run_attn(be, rng, rows, base, qh, heads, BF16, gate=heads == 3, paged=rows % 200 > 0, spread=3.0, seed=6)
+    check_attn(got, want, BF16, many=True)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.25, 1e-14])
+@pytest.mark.parametrize("rows,base", [(400, 300), (1000, 0)])
+def test_attn_many_rows_other_scales(be, rows, base, scale):
+    rng = np.random.default_rng(33)
+    got, want = run_attn(be, rng, rows, base, 8, 2, BF16, True, False, scale=scale)
+    check_attn(got, want, BF16, many=True)
+
+
+@pytest.mark.parametrize("rows", [1, 6, 300])
+@pytest.mark.parametrize("kinds", [(True, False), (False, True)], ids=["arena-plain", "plain-arena"])
+def test_attn_keys_and_values_in_caches_of_different_kinds(be, kinds, rows):
+    rng = np.random.default_rng(34)
+    heads, qh, base = 3, 6, 500
+    n, ctx = base + rows, base + rows + 77
+    with Bufs(be) as B:
+        ps = [Pair(be, B, heads, ctx, paged, seed=8) for paged in kinds]
+        k, v = draw_kv(rng, n, heads), draw_kv(rng, n, heads)
+        c = be.cmd_begin()
+        kr, vr = (QwRef(B.device(x.reshape(n, -1)), 0) for x in (k, v))
+        assert be.op_kv8_write(c, ps[0].kr, ps[1].vr, kr, vr, n, heads, HD, ctx, 0, heads * HD, F32)
+        ps[0].k.append(k, 0); ps[1].v.append(v, 0)
+        q = synth.bf16_round(rng.standard_normal((rows, qh, HD)).astype(np.float32))
+        qb, ob = B.device(to_io(q, BF16)), B.device(np.zeros((rows, qh, HD), np.uint16))
+        assert be.op_attn_kv8(c, QwRef(ob, 0), NULL_REF, QwRef(qb, 0), ps[0].kr, ps[1].vr, rows, qh, heads, HD, ctx, base, 1 / 16.0, HD, BF16)
+        be.cmd_wait(c); be.cmd_free(c)
+        got = np.empty((rows, qh, HD), np.uint16)
+        be.buf_download(ob, 0, got)
+        check_attn(from_io(got, BF16).astype(np.float64), M.attention(q, ps[0].k.values(0, n), ps[1].v.values(0, n), base, 1 / 16.0), BF16, many=rows > 16)
+
+
+@pytest.mark.parametrize("io", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,base", [(1, 40), (6, 900), (300, 700), (1000, 0)])
+def test_attn_nan_and_infinite_gates_stay_in_their_elements(be, io, rows, base):
+    rng = np.random.default_rng(35)
+    heads, qh = 2, 8
+    n = base + rows
+    with Bufs(be) as B:
+        p = Pair(be, B, heads, n, False)
+        c = be.cmd_begin()
+        assert p.append(c, B, draw_kv(rng, n, heads), draw_kv(rng, n, heads), 0, F32)
+        q = synth.bf16_round(rng.standard_normal((rows, qh, HD)).astype(np.float32))
+        g = synth.bf16_round(rng.standard_normal((rows, qh, HD)).astype(np.float32))
+        g[rows // 2, 3, 8] = np.inf
+        g[rows // 2, 3, 10] = -np.inf
+        g[0, 5, 200] = 300.0
+        want = M.attention(q, p.k.values(0, n), p.v.values(0, n), base, 1 / 16.0, np.clip(g, -700, 700))
+        bits = to_io(g, io)
+        bits = bits.view(np.uint32).copy() if io == F32 else bits.copy()
+        bits[rows // 2, 3, 6] = bits[rows // 2, 3, 13] = 0x7FC00000 if io == F32 else 0x7FC0
+        ob = B.device(np.zeros((rows, qh, HD), io_np(io)))
+        assert be.op_attn_kv8(c, QwRef(ob, 0), QwRef(B.device(bits), 0), QwRef(B.device(to_io(q, io)), 0), p.kr, p.vr, rows, qh, heads, HD, n, base, 1 / 16.0, HD, io)
+        be.cmd_wait(c); be.cmd_free(c)
+        got = np.empty((rows, qh, HD), io_np(io))
+        be.buf_download(ob, 0, got)
+        got = from_io(got, io).astype(np.float64)
+    odd = np.zeros(got.shape, bool)
+    odd[rows // 2, 3, [6, 13]] = True
+    assert np.array_equal(np.isnan(got), odd)
+    got[odd] = want[odd]
+    check_attn(got, want, io, many=rows > 16)
+
+
+@pytest.mark.parametrize("gate_stride", [HD, 260, 512])
+def test_attn_batch_of_many_rows(be, gate_stride):
+    """A tile kernel's launch per sequence, one after the other over the same scratch; 260: gate rows that the copy engine
+    does not take."""
+    rng = np.random.default_rng(36)
+    rows, qh, heads, bases = 150, 8, 2, [2500, 0, 1201]
+    ctx = 2800
+    with Bufs(be) as B:
+        ps = [Pair(be, B, heads, ctx, i != 1, seed=i) for i in range(3)]
+        c = be.cmd_begin()
+        qs, outs, gates, want = [], [], [], []
+        for p, b in zip(ps, bases):
+            assert p.append(c, B, draw_kv(rng, b + rows, heads), draw_kv(rng, b + rows, heads), 0, BF16)
+            q = synth.bf16_round(rng.standard_normal((rows, qh, HD)).astype(np.float32))
+            g = synth.bf16_round(rng.standard_normal((rows, qh, gate_stride)).astype(np.float32))
+            qs.append(QwRef(B.device(to_io(q, BF16)), 0))
+            gates.append(QwRef(B.device(to_io(g, BF16)), 0))
+            outs.append(QwRef(B.device(np.zeros((rows, qh, HD), np.uint16)), 0))
+            want.append(M.attention(q, p.k.values(0, b + rows), p.v.values(0, b + rows), b, 1 / 16.0, g[..., :HD]))
+        assert be.op_attn_kv8_batch(c, outs, gates, qs, [p.kr for p in ps], [p.vr for p in ps], bases, rows, qh, heads, HD, ctx, 1 / 16.0, gate_stride, BF16)
+        be.cmd_wait(c); be.cmd_free(c)
+        for o, w in zip(outs, want):
+            got = np.empty((rows, qh, HD), np.uint16)
+            be.buf_download(o.buf, 0, got)
+            check_attn(from_io(got, BF16).astype(np.float64), w, BF16, many=True)
+
+
+def test_call_refused_for_its_last_sequence_encodes_nothing(be):
+    rng = np.random.default_rng(37)
+    rows, qh, heads, ctx = 150, 8, 2, 400
+    with Bufs(be) as B:
+        ps = [Pair(be, B, heads, ctx, False) for _ in range(66)]
+        x = QwRef(B.device(rng.standard_normal((rows, heads * HD)).astype(np.float32)), 0)
+        q = QwRef(B.device(np.zeros((rows, qh, HD), np.uint16)), 0)
+        outs = [QwRef(B.device(np.zeros((rows, qh, HD), np.uint16)), 0) for _ in range(2)] + [QwRef(B.device(np.zeros(64, np.uint16)), 0)]
+        launches = be.launch_count()
+        c = be.cmd_begin()
+        assert not be.op_kv8_write_batch(c, [p.kr for p in ps], [p.vr for p in ps], [x] * 66, [x] * 65 + [NULL_REF], [0] * 66, 1, heads, HD, ctx, heads * HD, F32)
+        be.cmd_wait(c, check=False); be.cmd_free(c)
+        c = be.cmd_begin()
+        assert not be.op_attn_kv8_batch(c, outs, None, [q] * 3, [p.kr for p in ps[:3]], [p.vr for p in ps[:3]], [200] * 3, rows, qh, heads, HD, ctx, 0.1, HD, BF16)
+        be.cmd_wait(c, check=False); be.cmd_free(c)
+        assert be.launch_count() == launches
+
+
+def test_captured_prompt_replays_beside_an_eager_one(be):
+    """Many rows, keys in shares: the graph's partial sums and those of a call on another stream lie apart."""
+    import torch
+    rng = np.random.default_rng(38)
+    rows, qh, heads, base = 170, 8, 2, 2000
+    n = base + rows
+    with Bufs(be) as B:
+        p = Pair(be, B, heads, n, True)
+        c0 = be.cmd_begin()
+        assert p.append(c0, B, draw_kv(rng, n, heads), draw_kv(rng, n, heads), 0, F32)
+        be.cmd_wait(c0); be.cmd_free(c0)
+        k, v = p.k.values(0, n), p.v.values(0, n)
+        qs = [synth.bf16_round(rng.standard_normal((rows, qh, HD)).astype(np.float32)) for _ in range(3)]
+        want = [M.attention(q, k, v, base, 1 / 16.0) for q in qs]
+        t = [torch.from_numpy(q).to("cuda", torch.bfloat16) for q in qs]
+        live = t[0].clone()
+        outs = [torch.zeros(rows, qh, HD, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+        ref = lambda x: QwRef(be.buf_wrap_device(x.data_ptr(), x.numel() * 2), 0)  # noqa: E731
+        r_live, r_two, r_out = ref(live), ref(t[2]), [ref(o) for o in outs]
+        B.all += [r_live.buf, r_two.buf] + [r.buf for r in r_out]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        cs = [be.cmd_begin(s.cuda_stream) for s in streams]
+        call = lambda c, q, o: be.op_attn_kv8(c, o, NULL_REF, q, p.kr, p.vr, rows, qh, heads, HD, n, base, 1 / 16.0, HD, BF16)  # noqa: E731
+        assert call(cs[0], r_live, r_out[0])
+        be.cmd_wait(cs[0])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            assert call(cs[0], r_live, r_out[0])
+        live.copy_(t[1])
+        torch.cuda.synchronize()
+        for _ in range(10):
+            with torch.cuda.stream(streams[0]):
+                g.replay()
+            assert call(cs[1], r_two, r_out[1])
+        torch.cuda.synchronize()
+        be.cmd_wait(cs[1])
+        for o, w in zip(outs, want[1:]):
+            check_attn(o.float().cpu().numpy().astype(np.float64), w, BF16, many=True)
+        g.reset()
+        for c in cs:
+            be.cmd_free(c)
+
+
 def test_offsets_past_32_bits(be):
     """Codes that lie more than 4 GB into the buffer; the untouched positions are zeros and take their share."""
     rng = np.random.default_rng(28)
