@@ -56,7 +56,8 @@ qw_buf  qw_kv8_arena_alloc_in(qw_buf pool, int32_t n_layers, int32_t kv_heads, i
  * multiple of 16 bytes) at base_pos, like qw_op_kv_write.  A block that begins with this call takes its
  * exponent from the call's rows; one that holds rows already keeps its exponent, or moves to a larger
  * one and its codes with it.  A rewind needs nothing: rows past the new end are overwritten, and the
- * exponent of the block that is cut only stays larger than it would have to be.  A NaN is stored as
+ * exponent of the block that is cut only stays larger than it would have to be.  An append ends the
+ * cache: rows behind it do not follow when its block's exponent moves.  A NaN is stored as
  * zero and an infinity as the block's largest code; either is reported by qw_cmd_error after
  * qw_cmd_wait.  The batch form takes n_seq sequences of `rows` rows each in one launch per 64.  A cache
  * may appear only once in a call.  An append inside a graph capture needs its pages mapped before. */
@@ -73,13 +74,15 @@ bool    qw_op_kv8_read(qw_cmd c, qw_ref dst, qw_ref cache, int32_t pos0, int32_t
  * [0, base_pos + r] of kv head h / (q_heads / kv_heads).  q, out [rows, q_heads, 256], f32 or bf16; gate
  * a null ref, or element (r, h, d) at gate[(r*q_heads + h)*gate_stride + d], in the same type: out is
  * multiplied by its sigmoid.  f32 is carried through (operands as two fp16 parts, sums in f32: about
- * 1e-6); bf16 rounds the softmax weights to fp16, in calls of many rows to bf16.  Few rows (rows *
- * grouping <= 64) run as one split-KV launch for up to 64 sequences; many bf16 rows on the tcgen05
- * kernel over a bf16 copy of the visible positions in scratch (1 KB per position and kv head);
- * many f32 rows in chunks of the former.  Grouping at most 64 (f32: 32).  Positions from base_pos + rows
- * on may hold anything.  Partials and copies live in scratch of the command buffer: calls on one command
- * buffer follow one another, two that may run at once (two streams, two captured graphs) need two
- * command buffers, which live as long as the graphs captured on them. */
+ * 1e-6); bf16 rounds the softmax weights to fp16.  Up to 32 query rows per kv head (rows * grouping) run
+ * as one split-KV launch for up to 64 sequences; more of them, in bf16, as a tcgen05 launch per sequence or
+ * in chunks of the former, whichever should take less time; in f32 in chunks.  Grouping at most 32.
+ * Positions from base_pos + rows on may hold anything; a NaN code among the visible ones (qw_op_kv8_write
+ * stores none) makes the rows that see it NaN.  Query rows count as finite up to 2^100.  K and V may lie in
+ * caches of different kinds; sequences of a batch may share a cache, outputs may not.  Partial sums live in
+ * scratch of the command buffer: calls on one command buffer follow one another, two that may run at once
+ * (two streams, two captured graphs) need two command buffers, which live as long as the graphs captured on
+ * them. */
 bool    qw_op_attn_kv8(qw_cmd c, qw_ref out, qw_ref gate, qw_ref q, qw_ref kcache, qw_ref vcache, int32_t rows,
                        int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t max_ctx, int32_t base_pos,
                        float scale, int32_t gate_stride, qw_dtype io);

@@ -75,7 +75,11 @@ __device__ __forceinline__ int tile_row(const Kv8AttnParams &p, const int32_t *t
 // =======================================================================================
 // One CTA per (64-token block, head, K or V, sequence): the block's new rows are read once into registers, their
 // largest magnitude gives the exponent, and the codes leave as whole 256-byte rows.  A block that holds rows already
-// keeps its exponent unless the new rows need a larger one; then its old codes are moved there first.
+// keeps its exponent unless the new rows need a larger one; then its old codes are moved there first.  The exponent is
+// known only when the last of the 64 rows is, so a CTA is one trip to memory, a reduction and the stores; what bounds it
+// is that trip and, with few CTAs to an SM, how much of it is in flight: 4096 bf16 rows of
+// 4 heads, K and V (16.8 MB in, 8.4 MB out), 4.7 us, one row 2.0 us (a trip for the old exponent and the rows together, and
+// where the exponent grew one more for the old codes).
 constexpr int WR_THREADS = 512, WR_WARPS = WR_THREADS / 32, WR_ROWS = BLK / WR_WARPS;
 
 // Largest of `v` over the block; the same for every thread.
@@ -234,7 +238,8 @@ __global__ void __launch_bounds__(RD_THREADS) kv8_read_kernel(T *__restrict__ ds
 //
 // The products are turned over: S^T = K Q^T and O^T = V^T P^T, so that the cache is the 16-row operand of the tensor
 // op and the query rows are its eight columns.  With Q as the 16-row operand half of every op of a decode step would
-// multiply padding, and the running output would take twice the registers.  Query row i = r * gqa + g of the group:
+// multiply padding, and the running output would take twice the registers.  (tcgen05 has no use here: its smallest tile is
+// 64 rows, 6 of which a decode step of 24 heads over 4 would fill.)  Query row i = r * gqa + g of the group:
 // all query heads of the kv head, all rows of the call.
 //
 // Types.  fp16 tensor ops, because an e4m3 code is an fp16 number exactly.  bf16 rows are exact in fp16 after scaling
@@ -254,10 +259,7 @@ constexpr int TILE = 32;
 constexpr int ENTRY = TILE * 256;                    // K or V codes of a tile
 constexpr int BOX = TILE * 128;
 constexpr float W_SHIFT = 14.0f;
-#ifndef QW_KV8_SEG_COST
-#define QW_KV8_SEG_COST 8
-#endif
-constexpr int SEG_COST = QW_KV8_SEG_COST;
+constexpr int SEG_COST = 8;                          // what a segment costs beside its tiles, in tiles (see kv8_attn_plan)
 
 struct Where { int s, h, t; };                       // sequence, kv head, tile of the group
 
@@ -309,6 +311,9 @@ __device__ __forceinline__ void store_out(const Kv8AttnParams &p, const Kv8AttnS
 // =======================================================================================
 // A warp takes whole tiles: K in one 8 KB slot of its own, V in another, each refilled as soon as it is read, so that
 // the other's load runs under its arithmetic.  The running output is 64 registers a thread; twelve warps fit an SM.
+// Memory bounds the long calls: eight sequences of 32 K keys, 24 heads over 4 (537 MB) 91 us, 5.9 TB/s, of which a plain read
+// of the same bytes takes 79; one sequence of 262 K keys 49.7 us of 43.5.  The short ones are a chain of trips: 4 K keys
+// 8.7 us with the merge, of which the 8.4 MB take 1.3.
 constexpr int D_WARPS = 12, D_THREADS = D_WARPS * 32, D_NS = 2;
 constexpr int D_OFF_Q = D_WARPS * D_NS * ENTRY;
 constexpr int D_OFF_M = D_OFF_Q + 8192;                   // [warp][8]
@@ -703,7 +708,9 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
 // codes are widened once, however many rows there are) and each takes 128 dims of V for all 32 keys.  What they swap is
 // the weights, through shared memory.  The running maximum is the pair's and lags: it moves only when a score exceeds it
 // by more than 2^4 (the pair votes with the barrier that also guards the weights' buffer), so that most tiles need no
-// reduction over the lanes and no rescaling; the weights reach 2^15 then, which fp16 holds.
+// reduction over the lanes and no rescaling; the weights reach 2^15 then, which fp16 holds.  Four tokens of 24 heads over
+// 4 behind 32 K keys: 27.4 us, of which the 67 MB take 10.3.  What bounds it is the chain inside a tile (scores, vote,
+// weights, swap, products: about 3 us, four or five tiles to a pair) and 13 us of launch, first loads, sums and merge.
 constexpr float VF_LAG = 4.0f, VF_SHIFT = 11.0f;
 
 template <int NT, bool F32>

@@ -24,6 +24,11 @@
 // TMEM columns (512): O [0,256) fp32 | Q high [256,320) four dims a column | P [320,384) fp16 pairs | S [384,512) fp32.
 // With few tiles the keys are cut into shares, so that all SMs have work; a share leaves (m, l, O) per tile row, and
 // kv8_prefill_merge_kernel adds them up.  Every wait is bounded; tensor memory is always released.
+//
+// A step's products take about 2048 clocks of the tensor core; the softmax chain of a step (S out of tensor memory, maximum
+// over 128 keys, 64 exponentials a thread, P back) takes about 2800 and is what bounds it, and tensor memory is full with
+// one tile (O, Q, P and S are its 512 columns), so that little else runs under it.  Prompt of 4096 tokens, 16 heads over 4:
+// 138 us, 1.0 PFLOP/s of 2 x 2 x 256 operations per visible pair; 499 tokens of 24 heads behind 16 K: 177 us, 1.1.
 #include "qw_kernels.h"
 #include <algorithm>
 #include <cuda_fp16.h>

@@ -8,6 +8,9 @@
 // and reduced modulo 2 pi in 64 bits (error below 1e-9), and only the remainder goes to the 32-bit sine
 // and cosine.  Those cost more than the rotation itself, so a block works out the angles of one row once,
 // in shared memory, and uses them for all the heads it takes.
+//
+// Memory bounds it: 4096 rows of 24 heads x 256, bf16, interleaved, 18.0 us, of which the bytes take 15.4 (blocks of 256
+// threads with fewer vectors on their way: 20.8).  One row of 16 heads: 1.6 us, the launch.
 #include "qw_kernels.h"
 
 namespace qw {

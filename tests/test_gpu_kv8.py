@@ -7,8 +7,8 @@ rounding (to e4m3, ties to even) is defined.  Attention over the same codes:
         the norm of a row's error stays below 1e-5 of the row's norm.
   bf16  the output's rounding (half a step, 2^-8 of the value at most) plus the weights' rounding to fp16 (2^-11
         each, of either sign): 2^-8 + 2^-10 of the row's largest value.
-  bf16, many rows: the weights are rounded to bf16 (2^-8 each), as in the bf16 cache's prefill, with the bounds
-        that has in test_gpu_attn.py: 1e-2 of the row's largest value, 5e-3 in the norm."""
+  bf16, many rows: the bounds of the bf16 cache's prefill in test_gpu_attn.py, 1e-2 of the row's largest value and
+        5e-3 in the norm: enough for weights rounded to bf16 (2^-8 each)."""
 import numpy as np
 import pytest
 
