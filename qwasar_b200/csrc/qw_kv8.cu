@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
 // the weights, through shared memory.  The running maximum is the pair's and lags: it moves only when a score exceeds it
 // by more than 2^4 (the pair votes with the barrier that also guards the weights' buffer), so that most tiles need no
 // reduction over the lanes and no rescaling; the weights reach 2^15 then, which fp16 holds.  Four tokens of 24 heads over
-// 4 behind 32 K keys: 27.4 us, of which the 67 MB take 10.3.  What bounds it is the chain inside a tile (scores, vote,
+// 4 behind 32 K keys: 26.6 us, of which the 67 MB take 10.3.  What bounds it is the chain inside a tile (scores, vote,
 // weights, swap, products: about 3 us, four or five tiles to a pair) and 13 us of launch, first loads, sums and merge.
 constexpr float VF_LAG = 4.0f, VF_SHIFT = 11.0f;
 
@@ -811,23 +811,26 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
         RowRaw<F32> raw[PER];
 #pragma unroll
         for (int u = 0; u < PER; u++) raw[u] = fetch_q<F32>(p, sq, head0, valid, warp + u * Cfg::WARPS, lane);
+        // (only the first part of K is asked for at once: what is on its way to all SMs in front of the query rows holds them up)
+        int k1 = 0, v1 = 0;
         if (nt > 0) {
             rows_from(0);
-            const int k1 = __shfl_sync(0xffffffffu, win_k, 1), v1 = __shfl_sync(0xffffffffu, win_v, 1);
-            if (lane == 0) {
-                load_k(done, win_k);
-                load_v(done, win_v);
-                if (nt > 1) {
-                    load_k(done + 1, k1);
-                    if (VS == 2) load_v(done + 1, v1);
-                }
-            }
+            exps_from(0);
+            k1 = __shfl_sync(0xffffffffu, win_k, 1); v1 = __shfl_sync(0xffffffffu, win_v, 1);
+            if (lane == 0) load_k(done, win_k);
         }
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             const int row = warp + u * Cfg::WARPS;
             next_rows(p, w, sq, seg_t0, seg_n, T, hi, row, lane);
             if (row < ROWS) stage_q<F32>(p, raw[u], row, lane, smem + Cfg::OFF_Q, sm_sc + row);
+        }
+        if (nt > 0 && lane == 0) {
+            load_v(done, win_v);
+            if (nt > 1) {
+                load_k(done + 1, k1);
+                if (VS == 2) load_v(done + 1, v1);
+            }
         }
         if (threadIdx.x < ROWS) sm_lim[threadIdx.x] = (int)threadIdx.x < valid ? sq.base_pos + (int)threadIdx.x / p.gqa : n_keys - 1;
         __syncthreads();
@@ -848,7 +851,7 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
         for (int i = 0; i < nt; i++) {
             const int key0 = (seg_t0 + pair + i * PAIRS) * TILE;
             const uint32_t n_t = done + i;
-            if ((i & 31) == 0) exps_from(i);
+            if (i > 0 && (i & 31) == 0) exps_from(i);
             const int ex = __shfl_sync(0xffffffffu, win_e, i & 31);
             constexpr int AHEAD_V = VS == 2 ? 2 : 1;
             int nv = __shfl_sync(0xffffffffu, win_v, (i + 1) & 31);
