@@ -311,9 +311,9 @@ __device__ __forceinline__ void store_out(const Kv8AttnParams &p, const Kv8AttnS
 // =======================================================================================
 // A warp takes whole tiles: K in one 8 KB slot of its own, V in another, each refilled as soon as it is read, so that
 // the other's load runs under its arithmetic.  The running output is 64 registers a thread; twelve warps fit an SM.
-// Memory bounds the long calls: eight sequences of 32 K keys, 24 heads over 4 (537 MB) 91 us, 5.9 TB/s, of which a plain read
-// of the same bytes takes 79; one sequence of 262 K keys 49.7 us of 43.5.  The short ones are a chain of trips: 4 K keys
-// 8.7 us with the merge, of which the 8.4 MB take 1.3.
+// Memory bounds the long calls: eight sequences of 32 K keys, 24 heads over 4 (537 MB) 88 us, 6.1 TB/s, of which a plain read
+// of the same bytes takes 79; one sequence of 262 K keys 48.4 us of 43.5.  The short ones are a chain of trips: 4 K keys
+// 8.3 us with the merge, of which the 8.4 MB take 1.3.
 constexpr int D_WARPS = 12, D_THREADS = D_WARPS * 32, D_NS = 2;
 constexpr int D_OFF_Q = D_WARPS * D_NS * ENTRY;
 constexpr int D_OFF_M = D_OFF_Q + 8192;                   // [warp][8]
@@ -331,6 +331,10 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
 }
 __device__ __forceinline__ void lds128(uint32_t (&v)[4], uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
+}
+
+__device__ __forceinline__ void l2_box(const CUtensorMap *map, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 
 // Query row `row` of a group, 8 dims per lane, as it lies in memory.  A segment asks for its query rows BEFORE it asks for
@@ -357,6 +361,31 @@ __device__ __forceinline__ void prefetch_rows(const void *base, int io, size_t r
     const size_t el = io == DT_F32 ? 4 : 2;
     const uint8_t *at = reinterpret_cast<const uint8_t *>(base) + (row0_el + ((size_t)r * q_heads + hh) * row_stride_el) * el + lane * 8 * el;
     asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+}
+// In front of the wait for the kernel before this one: what the CTA asks for first is brought into L2, under that kernel's
+// tail.  Nothing is read here but page tables, which no kernel writes; a line that the kernel before still writes is in L2
+// either way.  (Eight sequences of 32 K keys 88.3 us against 91.2, 262 K keys 48.4 against 49.7, 4 K 8.3 against 8.7; four tokens
+// behind 32 K 26.0 against 26.7, in f32 31.5 against 33.1.)  A decode warp takes tiles whole
+// (ROWS_K 32), a verify warp 16 keys of K and 128 dims of V.
+template <int ROWS_K>
+__device__ __forceinline__ void warm_tile(const Kv8AttnParams &p, const Kv8AttnSeq &sq, int h, int tile, int k_rows0, int v_col0, int lane) {
+    const int key = tile * 32;
+    auto row_of = [&](const int32_t *table) {
+        if (!table) return h * p.max_ctx + key;
+        const int pg = __ldg(table + (size_t)h * p.pt_stride + key / QW_KV8_PAGE_TOKENS);
+        return pg < 0 ? -1 : pg * QW_KV8_PAGE_TOKENS + (key & (QW_KV8_PAGE_TOKENS - 1));
+    };
+    const int rk = row_of(sq.ktab), rv = row_of(sq.vtab);
+    const size_t e = (size_t)h * p.exp_stride + key / BLK;
+    if (lane == 0 && rk >= 0) {
+        l2_box(&p.maps[sq.kmap], 0, rk + k_rows0); l2_box(&p.maps[sq.kmap], 128, rk + k_rows0);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(sq.kexp + e));
+    }
+    if (lane == 0 && rv >= 0) {
+        if (ROWS_K == 32) { l2_box(&p.maps[sq.vmap], 0, rv); l2_box(&p.maps[sq.vmap], 128, rv); }
+        else { l2_box(&p.maps[sq.vmap], v_col0, rv); l2_box(&p.maps[sq.vmap], v_col0, rv + 16); }
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(sq.vexp + e));
+    }
 }
 // One warp stages a row: scaled below 2^14 and put where the B fragments are read: step 4 q + i takes dims
 // 64 q + 16 t + 4 i + {0, 1 | 2, 3} of row g in lane (g, t).  `frags`: per tile of eight rows 8 pairs of steps x 32 lanes x
@@ -431,14 +460,19 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
         tma_prefetch_desc(&p.maps[0]);
         tma_prefetch_desc(&p.maps[1]);
     }
+    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
+    Where w = locate(p, lo);
+    {
+        const Kv8AttnSeq &sq = p.seq[w.s];
+        if (warp < 8) prefetch_rows(sq.q, p.io, (size_t)w.h * p.gqa * 256, 256, sq.rows, p.gqa, p.q_heads, warp, lane);
+        if (warp < min(sq.n_tiles - w.t, hi - lo)) warm_tile<32>(p, sq, w.h, w.t + warp, 0, 0, lane);
+    }
     __syncthreads();
     pdl_wait();
     pdl_launch_next();
 
     uint8_t *ring = smem + warp * NS * ENTRY;
     full += warp * NS;
-    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
-    Where w = locate(p, lo);
     uint32_t phase = 0;                              // of both slots: K in slot 0, V in slot 1
 
     auto load = [&](const Kv8AttnSeq &sq, int row, int is_v) {       // lane 0
@@ -709,7 +743,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
 // the weights, through shared memory.  The running maximum is the pair's and lags: it moves only when a score exceeds it
 // by more than 2^4 (the pair votes with the barrier that also guards the weights' buffer), so that most tiles need no
 // reduction over the lanes and no rescaling; the weights reach 2^15 then, which fp16 holds.  Four tokens of 24 heads over
-// 4 behind 32 K keys: 26.6 us, of which the 67 MB take 10.3.  What bounds it is the chain inside a tile (scores, vote,
+// 4 behind 32 K keys: 26.0 us, of which the 67 MB take 10.3.  What bounds it is the chain inside a tile (scores, vote,
 // weights, swap, products: about 3 us, four or five tiles to a pair) and 13 us of launch, first loads, sums and merge.
 constexpr float VF_LAG = 4.0f, VF_SHIFT = 11.0f;
 
@@ -760,6 +794,15 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
         tma_prefetch_desc(&p.maps[0]);
         tma_prefetch_desc(&p.maps[1]);
     }
+    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
+    Where w = locate(p, lo);
+    {
+        const Kv8AttnSeq &sq = p.seq[w.s];
+#pragma unroll 1
+        for (int i = warp; i < ROWS; i += Cfg::WARPS) prefetch_rows(sq.q, p.io, (size_t)w.h * p.gqa * 256, 256, sq.rows, p.gqa, p.q_heads, i, lane);
+        // (the first tile only: with the second the merge kernel before this one waits longer than the loads gain)
+        if (pair < min(sq.n_tiles - w.t, hi - lo)) warm_tile<16>(p, sq, w.h, w.t + pair, 16 * half, 128 * half, lane);
+    }
     __syncthreads();
     pdl_wait();
     pdl_launch_next();
@@ -768,8 +811,6 @@ __global__ void __launch_bounds__(VfCfg<NT, F32>::THREADS, 1) kv8_verify_kernel(
     uint64_t *full_k = full + warp * NS, *full_v = full_k + 2;
     uint8_t *px = smem + Cfg::OFF_PX + pair * 2 * Cfg::PX;
     float *mx = reinterpret_cast<float *>(smem + Cfg::OFF_MX) + pair * 2 * ROWS;
-    const int lo = p.share[blockIdx.x], hi = p.share[blockIdx.x + 1];
-    Where w = locate(p, lo);
     uint32_t done = 0;                               // tiles of this pair before the current segment
 
     for (int T = lo; T < hi;) {
