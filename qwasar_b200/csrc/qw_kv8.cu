@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) kv8_decode_kernel(const __grid_c
 // by more than 2^4 (the pair votes with the barrier that also guards the weights' buffer), so that most tiles need no
 // reduction over the lanes and no rescaling; the weights reach 2^15 then, which fp16 holds.  Four tokens of 24 heads over
 // 4 behind 32 K keys: 26.0 us, of which the 67 MB take 10.3.  What bounds it is the chain inside a tile (scores, vote,
-// weights, swap, products: about 3 us, four or five tiles to a pair) and 13 us of launch, first loads, sums and merge.
+// weights, swap, products: about 3 us, four or five tiles to a pair) and 12 us of launch, first loads, sums and merge.
 constexpr float VF_LAG = 4.0f, VF_SHIFT = 11.0f;
 
 template <int NT, bool F32>
